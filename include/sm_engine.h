@@ -316,6 +316,130 @@ int sm_gemv_noalloc(const sm_dweight* w, const float* x_dev, float* y_dev, uint6
 int sm_gemv_noalloc_status(void* stream);
 
 /* ------------------------------------------------------------------------
+ * One serving step over an 8-bit paged KV cache, for hosts that batch their
+ * own requests and own all device memory. No reference counterpart: the
+ * reference's SeqState holds f32 vectors and its caller walks one sequence at
+ * a time. A step is sm_kv_plan (pages and slots of the new tokens), then for
+ * each layer sm_kv8_append and sm_kv8_attend, then sm_draw.
+ *
+ * Every *_dev argument is memory of the current device (checked). The calls
+ * only launch work on `stream` (a cudaStream_t of that device, NULL = the
+ * default stream) and can be captured in a CUDA graph; they neither allocate
+ * nor wait. What a call reads must stay unchanged, and what it writes must
+ * not be used by other work, until it has run. Strides and alignment: rows
+ * (K, V, q, out) begin at multiples of 16 bytes.
+ * Types of rows and logits are ggml codes: F32 (0), F16 (1), BF16 (30).
+ * ---------------------------------------------------------------------- */
+#define SM_KV8_PAGE 32
+#define SM_KV8_E4M3 0u /* codes are 8-bit floats, 4 exponent and 3 mantissa bits, largest 448 */
+#define SM_KV8_I8 1u   /* codes are signed integers, -127..127 */
+
+/* One layer's cache. A page holds 32 consecutive positions of one sequence;
+ * a value of it is code * scale, with one scale for a page's K rows of a KV
+ * head and one for its V rows. n_pages is the pool's size; a sequence's pages
+ * are the entries of its row of a block table, in the order of its positions.
+ * All layers of a model can share block tables and slots. */
+typedef struct {
+  void* codes_dev;   /* [n_pages][n_kv_heads][2 (K, V)][32][head_dim] bytes, 16-byte aligned */
+  float* scales_dev; /* [n_pages][n_kv_heads][2 (K, V)], 8-byte aligned */
+  uint64_t n_pages;
+  uint32_t n_kv_heads; /* 1..1024 */
+  uint32_t head_dim;   /* a multiple of 16, 16..128 */
+  uint32_t format;     /* SM_KV8_* */
+  uint32_t reserved;
+} sm_kv8;
+
+/* Pages, slots and rows of a step, from lengths in device memory. Sequence i
+ * (i < n_seqs <= 16384) holds lens_dev[i] positions and gets add_dev[i] new
+ * ones; the new tokens of all sequences are rows 0, 1, ... in order, of n_rows
+ * rows in all (more than the sum of add_dev: the last ones are padding).
+ * - table_dev [n_seqs][table_ld]: the entries of pages that sequence i now
+ *   needs in addition are written, the others kept. Pages are taken from the
+ *   end of free_dev (n_free_dev[0] page ids), in the order of the sequences;
+ *   free_dev itself is not written.
+ * - first_dev [n_seqs + 1]: the row of sequence i's first new token; the last
+ *   entry is their number (2^31 - 1 where it would be more).
+ * - slots_dev [n_rows]: page * 32 + offset of the row's position, -1 for a
+ *   padding row and for rows of a refused sequence (and where the table's own
+ *   entry is negative). pos_dev, seq_dev [n_rows] (each may be NULL): the
+ *   row's position in its sequence (-1 like slots) and its sequence (-1 for a
+ *   padding row).
+ * - lens_out_dev [n_seqs] (not lens_dev itself): the new length, or -1 if the
+ *   sequence is refused: its length or add is negative, it would exceed its
+ *   table row or n_rows, or it needs pages and the pages that it and the
+ *   sequences before it need are more than the list has. A refused sequence
+ *   keeps its place in first_dev (a negative add counts as 0), takes no page,
+ *   and its lens_out of -1 makes its rows attend to nothing.
+ * - status_dev [2]: pages left in the free list, number of refused sequences. */
+int sm_kv_plan(uint64_t n_seqs, const int32_t* lens_dev, const int32_t* add_dev, int32_t* table_dev, uint64_t table_ld,
+               const int32_t* free_dev, const int32_t* n_free_dev, uint64_t n_rows, int32_t* lens_out_dev,
+               int32_t* first_dev, int64_t* slots_dev, int32_t* pos_dev, int32_t* seq_dev, int32_t* status_dev,
+               void* stream);
+
+/* Quantises n_rows rows of K and V ([n_kv_heads][head_dim] each, ld_k / ld_v
+ * elements apart, 0: contiguous) into the cache; row t goes to slots_dev[t]
+ * (page * 32 + offset). Rows with a slot that is negative or behind the pool
+ * are skipped. A page's rows are consecutive rows of one call with slots that
+ * rise by one, beginning at offset 0 or behind the rows the page already
+ * holds; what a call leaves in a page that it gets twice, or with gaps, is
+ * unspecified (other pages are not touched).
+ * Scales are powers of two: the smallest (2^-100 at least) at which the
+ * largest magnitude of the page's rows of that head fits the format. A page
+ * that begins at offset 0 forgets what it held. Rows added to a page keep its
+ * scale unless they need a larger one; the codes already there are then
+ * rounded again, to the larger scale. Codes are rounded to nearest even. A row
+ * that is not finite makes the scale of its page and head NaN, hence all those
+ * values. */
+int sm_kv8_append(const sm_kv8* c, const void* k_dev, const void* v_dev, uint32_t type, uint64_t n_rows, uint64_t ld_k,
+                  uint64_t ld_v, const int64_t* slots_dev, void* stream);
+
+/* Scratch of sm_kv8_attend on the current device: partial results of
+ * sequences that several CTAs share. One serves all calls that run one after
+ * another; calls that may overlap (two streams, two graphs) need one each. */
+typedef struct sm_kv8_ws sm_kv8_ws;
+int sm_kv8_ws_new(sm_kv8_ws** out);
+int sm_kv8_ws_free(sm_kv8_ws* w);
+
+/* Attention of n_rows query rows ([n_heads][head_dim], ld_q elements apart,
+ * 0: contiguous) over the cache; query head h reads KV head
+ * h / (n_heads / n_kv_heads). Rows first_dev[s] .. first_dev[s + 1] - 1 are
+ * the last positions of sequence s, which holds lens_dev[s] positions (their
+ * own K and V included) in the pages table_dev[s * table_ld ...]. A row sees
+ * the positions up to its own, with window > 0 only the last `window` of
+ * them. out (like q, ld_out) is the softmax(scale q K)-weighted sum of V; a
+ * row that sees nothing (a length of 0 or -1 among them) gets zeros, and rows
+ * behind first_dev[n_seqs] are left as they were. Positions whose page id is
+ * not in the pool take no part. Scales may be any finite values >= 0.
+ * Products and sums are f32; scores and weights enter the tensor cores with
+ * 22 bits for F32 rows and as f16 for F16 and BF16 rows. */
+int sm_kv8_attend(const sm_kv8* c, sm_kv8_ws* ws, const void* q_dev, void* out_dev, uint32_t type, uint64_t n_rows,
+                  uint32_t n_heads, uint64_t ld_q, uint64_t ld_out, uint64_t n_seqs, const int32_t* lens_dev,
+                  const int32_t* first_dev, const int32_t* table_dev, uint64_t table_ld, float scale, uint32_t window,
+                  void* stream);
+
+/* How sm_draw samples one row. */
+typedef struct {
+  float temperature; /* > 0; else greedy: the largest logit, the lowest index among equals */
+  int32_t top_k;     /* keep the k largest (equal ones: lowest indices first); <= 0: all */
+  float top_p;       /* of those, keep while the probability before is below top_p of theirs (the first always); >= 1: all */
+  float min_p;       /* of those, keep probabilities of at least min_p times the largest (the first always); <= 0: all */
+} sm_draw_params;
+
+/* Draws a token for each of n_rows <= 65536 rows of `vocab` (1..524288) device
+ * logits, ld elements apart (0: vocab), with the row's own parameters and
+ * uniform number u in [0, 1): the first kept index, in the vocabulary's order,
+ * at which the kept probabilities sum to more than u of their total. mask_dev
+ * (may be NULL; ld as the logits): 0 = forbidden. NaN and -inf logits are
+ * forbidden too, +inf counts as the largest float. A row with nothing left
+ * gets token -1 and log probability -inf. logprobs_dev (may be NULL): natural
+ * log of the token's probability among the kept ones (0 when greedy). Weights
+ * are summed exactly in 64 bits: a draw does not depend on the order of sums.
+ * Not sm_sample: that one reproduces the reference's f32 sampler and its RNG
+ * bit for bit, on host logits. */
+int sm_draw(const void* logits_dev, uint32_t type, uint64_t n_rows, uint64_t ld, uint64_t vocab, const uint8_t* mask_dev,
+            const sm_draw_params* params_dev, const float* u_dev, int32_t* tokens_dev, float* logprobs_dev, void* stream);
+
+/* ------------------------------------------------------------------------
  * Synthetic GGUF models (the stand-in for real model files). Shapes and
  * metadata keys follow qwen2.rs:30-63; values are seeded N(0, weight_std).
  * ---------------------------------------------------------------------- */

@@ -26,6 +26,7 @@ LIB_PATH = os.path.join(_HERE, "libsmotor.so")
 
 # ggml type codes (crates/s-gguf/src/types.rs)
 F32, Q5_0, Q8_0, Q4_K, Q6_K = 0, 6, 8, 12, 14
+F16, BF16 = 1, 30
 BLOCK = {Q4_K: (256, 144), Q6_K: (256, 210), Q5_0: (32, 22), Q8_0: (32, 34), F32: (1, 4)}
 
 
@@ -62,6 +63,19 @@ ERR_PEER = 9  # SM_ERR_PEER
 
 class sm_sampler(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int64), ("top_p", C.c_float)]
+
+
+class sm_kv8(C.Structure):
+    _fields_ = [("codes_dev", C.c_void_p), ("scales_dev", C.c_void_p), ("n_pages", C.c_uint64),
+                ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("format", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class sm_draw_params(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
+
+
+KV8_PAGE = 32
+KV8_E4M3, KV8_I8 = 0, 1  # SM_KV8_*
 
 
 class sm_gen_params(C.Structure):
@@ -149,6 +163,12 @@ SIGNATURES = {
     "sm_model_embedding": (C.c_int, [P, U32, C.POINTER(C.c_float)]),
     "sm_gemv_status": (C.c_int, [P, P]),
     "sm_gemv_noalloc_status": (C.c_int, [P]),
+    "sm_kv_plan": (C.c_int, [U64, P, P, P, U64, P, P, U64, P, P, P, P, P, P, P]),
+    "sm_kv8_append": (C.c_int, [C.POINTER(sm_kv8), P, P, U32, U64, U64, U64, P, P]),
+    "sm_kv8_ws_new": (C.c_int, [C.POINTER(P)]),
+    "sm_kv8_ws_free": (C.c_int, [P]),
+    "sm_kv8_attend": (C.c_int, [C.POINTER(sm_kv8), P, P, P, U32, U64, U32, U64, U64, U64, P, P, P, U64, C.c_float, U32, P]),
+    "sm_draw": (C.c_int, [P, U32, U64, U64, U64, P, P, P, P, P, P]),
     "sm_synth_preset": (C.c_int, [C.c_int, C.POINTER(sm_synth_spec)]),
     "sm_synth_size": (C.c_int, [C.POINTER(sm_synth_spec), PU64]),
     "sm_synth_write": (C.c_int, [C.POINTER(sm_synth_spec), C.c_char_p, C.c_int]),
@@ -633,6 +653,67 @@ class DWeight:
 def gemv_noalloc_status(stream: int = 0) -> None:
     """Raises if a bounded wait in an earlier gemv_noalloc() on the current device gave up."""
     _check(lib().sm_gemv_noalloc_status(C.c_void_p(stream)))
+
+
+# -------------------------------------------- 8-bit paged KV serving step ----
+def kv_plan(n_seqs: int, lens: int, add: int, table: int, table_ld: int, free: int, n_free: int, n_rows: int,
+            lens_out: int, first: int, slots: int, status: int, pos: int = 0, seq: int = 0, stream: int = 0) -> None:
+    """sm_kv_plan over device pointers: pages, slots and rows of a step's new
+    tokens from the sequences' lengths (pos and seq may be 0)."""
+    _check(lib().sm_kv_plan(n_seqs, lens, add, table, table_ld, free, n_free, n_rows, lens_out, first, slots, pos, seq,
+                            status, stream))
+
+
+class Kv8Workspace:
+    """Scratch of Kv8Cache.attend on the current device (sm_kv8_ws): one for
+    calls that follow one another, one each for calls that may overlap."""
+
+    def __init__(self):
+        out = C.c_void_p()
+        _check(lib().sm_kv8_ws_new(C.byref(out)))
+        self.h = out
+
+    def free(self) -> None:
+        if self.h:
+            lib().sm_kv8_ws_free(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class Kv8Cache:
+    """One layer's 8-bit paged KV cache in the caller's device memory (sm_kv8):
+    codes [n_pages][n_kv_heads][2][32][head_dim], scales [n_pages][n_kv_heads][2]."""
+
+    def __init__(self, codes: int, scales: int, n_pages: int, n_kv_heads: int, head_dim: int, fmt: int = KV8_E4M3):
+        self.c = sm_kv8(codes, scales, n_pages, n_kv_heads, head_dim, fmt, 0)
+        self._ref = C.byref(self.c)
+
+    def append(self, k: int, v: int, dtype: int, n_rows: int, slots: int, ld_k: int = 0, ld_v: int = 0,
+               stream: int = 0) -> None:
+        """Quantise K and V rows into the pages of their slots (sm_kv8_append)."""
+        _check(lib().sm_kv8_append(self._ref, k, v, dtype, n_rows, ld_k, ld_v, slots, stream))
+
+    def attend(self, ws: Kv8Workspace, q: int, out: int, dtype: int, n_rows: int, n_heads: int, n_seqs: int, lens: int,
+               first: int, table: int, table_ld: int, scale: Optional[float] = None, window: int = 0, ld_q: int = 0,
+               ld_out: int = 0, stream: int = 0) -> None:
+        """Causal attention of the rows over their sequences' pages
+        (sm_kv8_attend); scale None = 1 / sqrt(head_dim)."""
+        if scale is None:
+            scale = self.c.head_dim ** -0.5
+        _check(lib().sm_kv8_attend(self._ref, ws.h, q, out, dtype, n_rows, n_heads, ld_q, ld_out, n_seqs, lens, first,
+                                   table, table_ld, scale, window, stream))
+
+
+def draw(logits: int, dtype: int, n_rows: int, vocab: int, params: int, u: int, tokens: int, logprobs: int = 0,
+         mask: int = 0, ld: int = 0, stream: int = 0) -> None:
+    """sm_draw over device pointers: a token a row from its logits, its
+    sm_draw_params and its uniform number (logprobs and mask may be 0)."""
+    _check(lib().sm_draw(logits, dtype, n_rows, ld, vocab, mask, params, u, tokens, logprobs, stream))
 
 
 # ------------------------------------------------------------- synthetic ----

@@ -1,0 +1,135 @@
+"""The 8-bit paged KV cache and sm_draw without a device: arguments that the
+entry points refuse before they touch a GPU, and the 64-bit statements the GPU
+tests compare with (tests/kv8_ref.py) against each other and by hand."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import kv8_ref as ref
+import smotor
+
+ARG = 1  # SM_ERR_ARG
+OK = 0x1000  # an aligned non-null address; nothing reads it
+
+
+def refused(call):
+    with pytest.raises(smotor.EngineError) as e:
+        call()
+    assert e.value.status == ARG, str(e.value)
+
+
+def plan(**kw):
+    a = dict(n_seqs=2, lens=OK, add=OK, table=OK, table_ld=4, free=OK, n_free=OK, n_rows=2, lens_out=OK + 4096, first=OK,
+             slots=OK, status=OK)
+    a.update(kw)
+    smotor.kv_plan(**a)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(n_seqs=16385), dict(n_rows=1 << 31), dict(table_ld=1 << 31), dict(lens_out=OK), dict(lens=0), dict(add=0),
+    dict(table=0), dict(n_free=0), dict(lens_out=0), dict(first=0), dict(slots=0), dict(status=0), dict(lens=OK + 2),
+    dict(slots=OK + 4)])
+def test_plan_refuses(kw):
+    refused(lambda: plan(**kw))
+
+
+def cache(**kw):
+    a = dict(codes=OK, scales=OK, n_pages=4, n_kv_heads=2, head_dim=64, fmt=smotor.KV8_E4M3)
+    a.update(kw)
+    return smotor.Kv8Cache(**a)
+
+
+@pytest.mark.parametrize("kw", [dict(fmt=2), dict(head_dim=0), dict(head_dim=24), dict(head_dim=144), dict(n_kv_heads=0),
+                                dict(n_kv_heads=1025), dict(n_pages=0), dict(n_pages=1 << 31), dict(codes=0),
+                                dict(codes=OK + 8)])
+def test_cache_descriptions_refused(kw):
+    refused(lambda: cache(**kw).append(OK, OK, smotor.F32, 1, OK))
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=smotor.Q8_0), dict(n_rows=1 << 31), dict(ld_k=64), dict(ld_v=130),
+                                dict(ld_k=1 << 32)])
+def test_append_refuses(kw):
+    a = dict(k=OK, v=OK, dtype=smotor.F32, n_rows=1, slots=OK)
+    a.update(kw)
+    refused(lambda: cache().append(**a))
+
+
+def test_append_of_no_rows_is_nothing():
+    cache().append(0, 0, smotor.F32, 0, 0)
+
+
+class NoWorkspace:
+    h = None
+
+
+def test_attend_refuses_without_workspace():
+    refused(lambda: cache().attend(NoWorkspace(), OK, OK, smotor.F32, 1, 4, 1, OK, OK, OK, 1))
+
+
+def draw(**kw):
+    a = dict(logits=OK, dtype=smotor.F32, n_rows=1, vocab=100, params=OK, u=OK, tokens=OK)
+    a.update(kw)
+    smotor.draw(**a)
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=smotor.Q6_K), dict(vocab=0), dict(vocab=524289), dict(ld=99),
+                                dict(n_rows=65537), dict(logits=0), dict(logits=OK + 2)])
+def test_draw_refuses(kw):
+    refused(lambda: draw(**kw))
+
+
+def test_draw_of_no_rows_is_nothing():
+    draw(n_rows=0, logits=0, params=0, u=0, tokens=0)
+
+
+def test_null_structs_and_outputs_refused():
+    assert smotor.lib().sm_kv8_append(None, OK, OK, 0, 1, 0, 0, OK, None) == ARG
+    assert smotor.lib().sm_kv8_ws_new(None) == ARG
+    assert smotor.lib().sm_kv8_ws_free(None) == 0
+
+
+# ------------------------------------------------- the statements themselves ----
+def test_e4m3_against_torch():
+    torch = pytest.importorskip("torch")
+    codes = torch.arange(256, dtype=torch.uint8)
+    want = codes.view(torch.float8_e4m3fn).float().numpy().astype(np.float64)
+    assert np.array_equal(ref.E4M3, want, equal_nan=True)
+    r = np.random.default_rng(0)
+    x = np.concatenate([r.normal(0, 100, 20000), r.normal(0, 0.01, 20000), ref.E4M3[:126] + np.diff(ref.E4M3[:127]) / 2,
+                        [0.0, -0.0, 448.0, -448.0, 2.0**-10, 2.0**-11, 2.0**-12]])
+    x = np.clip(x, -448, 448).astype(np.float32)
+    got = ref.encode(x.astype(np.float64), "e4m3")
+    assert np.array_equal(got, torch.from_numpy(x).to(torch.float8_e4m3fn).view(torch.uint8).numpy())
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "i8"])
+def test_page_scale_is_the_smallest(fmt):
+    r = np.random.default_rng(1)
+    top = np.abs(r.normal(0, 1, 200)) * 2.0 ** r.integers(-80, 100, 200)
+    top = np.concatenate([top, ref.TOP[fmt] * 2.0 ** r.integers(-60, 60, 20), [0.0]])
+    s = ref.page_scale(top, fmt)
+    assert np.all(top <= ref.TOP[fmt] * s) and np.all((top > ref.TOP[fmt] * s / 2) | (s == 2.0**-100))
+
+
+def test_plan_by_hand():
+    table = np.full((3, 3), -1)
+    table[0, 0], table[2, 0] = 7, 8
+    t, lens_out, first, slots, pos, seq, status = ref.plan([31, 0, 32], [2, 0, 1], table, [4, 5, 6], 3, 5)
+    assert t[0, 1] == 6 and t[2, 1] == 5 and list(lens_out) == [33, 0, 33] and list(first) == [0, 2, 2, 3]
+    assert list(slots) == [7 * 32 + 31, 6 * 32, 5 * 32, -1, -1] and list(pos) == [31, 32, 32, -1, -1]
+    assert list(seq) == [0, 0, 2, -1, -1] and list(status) == [1, 0]
+
+
+def test_draw_by_hand():
+    x = np.log(np.array([1.0, 4.0, 2.0, 1.0]))
+    assert [ref.draw(x, 1, 0, 1, 0, u)[0] for u in (0, 0.12, 0.13, 0.62, 0.63, 0.99)] == [0, 0, 1, 1, 2, 3]
+    assert [ref.draw(x, 1, 2, 1, 0, u)[0] for u in (0, 0.66, 0.67)] == [1, 1, 2]
+    assert [ref.draw(x, 1, 0, 0.5, 0, u)[0] for u in (0, 0.99)] == [1, 1]
+    assert [ref.draw(x, 1, 0, 0.51, 0, u)[0] for u in (0, 0.99)] == [1, 2]
+    assert [ref.draw(x, 1, 0, 1, 0.4, u)[0] for u in (0, 0.99)] == [1, 2]
+    assert ref.draw(x, 0, 0, 1, 0, 0.5) == (1, 0.0) and ref.draw(x, 1, 0, 1, 0, 0.5, np.zeros(4))[0] == -1
+
+
+def test_the_structs_have_the_headers_sizes():
+    assert C.sizeof(smotor.sm_kv8) == 40 and C.sizeof(smotor.sm_draw_params) == 16
