@@ -342,7 +342,8 @@ cudaError_t draw_typed(const DrawArgs& a, cudaStream_t st) {
   const uint32_t chunk = ((a.vocab + cl - 1) / cl + 7) / 8 * 8;
   const size_t smem = sizeof(Shared) + (size_t)chunk * 4;
   auto* kern = draw_kernel<T>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(Shared) + 40 * 1024 * 4 + 64));
+  static SmemOnce once;
+  cudaError_t e = once.allow((const void*)kern, (int)(sizeof(Shared) + 40 * 1024 * 4 + 64));
   if (e == cudaSuccess && cl > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};

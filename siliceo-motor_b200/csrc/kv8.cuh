@@ -5,7 +5,22 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace sm {
+
+// A kernel's shared memory limit, raised once on each device.
+struct SmemOnce {
+  std::atomic<uint64_t> done{0};
+  cudaError_t allow(const void* kern, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done.load(std::memory_order_relaxed) >> dev & 1)) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return e;
+  }
+};
 
 // Positions of a page: the engine's own page size (device.cuh).
 constexpr uint32_t KV8_PAGE = 32;
@@ -70,9 +85,19 @@ cudaError_t launch_kv8_plan(const Kv8PlanArgs& a, cudaStream_t st);
 // ld_k, ld_v: elements between rows.
 cudaError_t launch_kv8_append(const Kv8& c, const void* k, const void* v, uint32_t type, uint32_t n_rows, uint64_t ld_k,
                               uint64_t ld_v, const int64_t* slots, cudaStream_t st);
-uint64_t kv8_attn_part_floats(uint32_t sms);
-uint32_t kv8_attn_counters(uint32_t sms);
-cudaError_t launch_kv8_attn(const Kv8AttnArgs& a, uint32_t type, uint32_t sms, cudaStream_t st);
+// Streaming attention (kv8_attn.cuh), one translation unit a row type.
+constexpr uint32_t KV8_MAX_HD = 128;
+constexpr uint32_t KV8_PART_FLOATS = 16 * (KV8_MAX_HD + 2);  // a partial result of up to 16 rows: o, then m and l
+inline uint64_t kv8_attn_part_floats(uint32_t sms) { return (uint64_t)sms * 2 * KV8_PART_FLOATS; }
+inline uint32_t kv8_attn_counters(uint32_t sms) { return sms; }
+cudaError_t launch_kv8_attn_f32(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st);
+cudaError_t launch_kv8_attn_f16(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st);
+cudaError_t launch_kv8_attn_bf16(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st);
+inline cudaError_t launch_kv8_attn(const Kv8AttnArgs& a, uint32_t type, uint32_t sms, cudaStream_t st) {
+  return type == ACT_F32   ? launch_kv8_attn_f32(a, sms, st)
+         : type == ACT_F16 ? launch_kv8_attn_f16(a, sms, st)
+                           : launch_kv8_attn_bf16(a, sms, st);
+}
 // Largest vocabulary launch_draw takes.
 constexpr uint32_t DRAW_MAX_VOCAB = 1u << 19;
 cudaError_t launch_draw(const DrawArgs& a, cudaStream_t st);
