@@ -50,8 +50,14 @@ template <typename T, uint32_t HDV, uint32_t NR>
 struct Shape {
   static constexpr bool SPLIT = sizeof(T) == 4;
   static constexpr uint32_t WARPS = NR == 8 ? (SPLIT && HDV > 64 ? 12 : 16) : (HDV > 64 ? 12 : 16);
-  static constexpr uint32_t VALUES = TILE * HDV, SCALES = 2 * VALUES;  // K's codes, V's, then every lane's copy of the scales
-  static constexpr uint32_t STAGE = SCALES + 32 * 8;
+  static constexpr uint32_t VALUES = TILE * HDV, SCALES = 2 * VALUES;  // a page: K's codes, V's, then the scales
+  static constexpr uint32_t STAGE = SCALES + 16;
+  // Byte offset of 16-byte column c of row r. The columns of each 128 bytes are exchanged by the row, so that
+  // the 8 lanes of a shared-memory phase, (g, t) with two g for K and with four rows 2t for V, meet 8 of them.
+  static __device__ uint32_t at(uint32_t r, uint32_t c) {
+    if (HDV == 128) return r * 128 + ((c ^ ((r >> 1 & 3) << 1) ^ ((r & 1) << 2)) << 4);
+    return (r >> 1) * 128 + ((((r & 1) << 2 | c) ^ ((r >> 1 & 3) << 1)) << 4);
+  }
   static constexpr uint32_t PART = NR * HDV * 4, ML = NR * 2 * 4;  // a partial result: o, then m and l
   static constexpr uint32_t RING = STAGE > PART + ML ? STAGE : PART + ML;
   static constexpr uint32_t WARP = RING + PART + ML;  // the second partial lies over the page, done by then
@@ -78,12 +84,12 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ uint2 lds8(uint32_t a) {
   uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
   return v;
 }
 // An 8 x 8 matrix of f16 across the warp, transposed.
@@ -196,6 +202,11 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
   const int64_t share = max((total + n_warps - 1) / n_warps, (int64_t)2);
   const int64_t x_begin = min(total, ((int64_t)blockIdx.x * WARPS + warp) * share), x_end = min(total, x_begin + share);
 
+  if (!FULL) {  // columns behind hd stay zero
+    for (uint32_t i = lane * 16; i < L::SCALES; i += 512)
+      *reinterpret_cast<uint4*>((char*)attn_smem4 + warp * L::WARP + i) = make_uint4(0, 0, 0, 0);
+    __syncwarp();
+  }
   if (x_begin < x_end) {
     // ---- where this warp's share begins ----
     uint32_t seq = 0;
@@ -241,7 +252,6 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
       int32_t page0 = tile;
       auto page_id = [&](int32_t pg) { return (uint64_t)pg < a.table_ld && pg < tile_stop ? (uint32_t)table[pg] : ~0u; };
       uint32_t ids = page_id(page0 + (int32_t)lane), ids_next = page_id(page0 + 32 + (int32_t)lane);
-      const uint32_t k_off = g * hd + 16 * t, v_off = 32 * hd + 2 * t * hd + (HDV / 8) * g;
       auto find = [&](int32_t pg) -> uint32_t {
         if (pg - page0 >= 32) {
           page0 += 32;
@@ -250,34 +260,29 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
         }
         return __shfl_sync(~0u, ids, (pg - page0) & 31);
       };
+      // K's or V's 32 rows of a page, 512 consecutive bytes a warp and step. Rows at and behind
+      // `n` arrive as zeros: behind a sequence's end lies anything.
+      auto copy_rows = [&](uint32_t dst, const uint8_t* src, int32_t n) {
+        const uint32_t cpr = hd / 16;
+#pragma unroll
+        for (uint32_t i = 0; i < HDV / 16; i++) {
+          if (!FULL && i >= cpr) break;
+          const uint32_t at = i * 32 + lane, row = FULL ? at / (HDV / 16) : at / cpr, col = at - row * (FULL ? HDV / 16 : cpr);
+          copy16(dst + L::at(row, col), src + at * 16, (int32_t)row < n);
+        }
+      };
       auto fetch_k = [&](int32_t pg, uint32_t id) {  // an id outside the pool: no such page, its positions take no part
         if (pg < tile_stop && id < a.c.n_pages) {
           const uint64_t at = ((uint64_t)id * a.c.heads + head) * 2;
-          const uint8_t* kp = a.c.codes + at * KV8_PAGE * hd;
-#pragma unroll
-          for (int n = 0; n < 4; n++)
-#pragma unroll
-            for (int sg = 0; sg < SEG; sg++) {
-              const bool in = FULL || 64 * sg + 16 * t < hd;
-              copy16(ring + lane * 16 + (n * SEG + sg) * 512, kp + (in ? k_off + n * 8 * hd + 64 * sg : 0), in);
-            }
-          copy8(ring + L::SCALES + lane * 8, a.c.scales + at, true);
+          copy_rows(ring, a.c.codes + at * KV8_PAGE * hd, KV8_PAGE);
+          if (lane == 0) copy8(ring + L::SCALES, a.c.scales + at, true);
         }
         copy_commit();
       };
       auto fetch_v = [&](int32_t pg, uint32_t id) {
-        if (pg < tile_stop && id < a.c.n_pages) {
-          const uint8_t* kp = a.c.codes + ((uint64_t)id * a.c.heads + head) * 2 * KV8_PAGE * hd;
-          const bool whole = (pg + 1) * (int32_t)TILE <= sq.len;  // behind the end lies anything
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const uint32_t p = (i & 1) + 8 * (i >> 1);
-            const bool in = (FULL || (HDV / 8) * g < hd) && (whole || pg * (int32_t)TILE + (int32_t)(p + 2 * t) < sq.len);
-            const uint8_t* src = kp + (in ? v_off + p * hd : 0);
-            if constexpr (HDV == 128) copy16(ring + L::VALUES + lane * 16 + i * 512, src, in);
-            else copy8(ring + L::VALUES + lane * 8 + i * 256, src, in);
-          }
-        }
+        if (pg < tile_stop && id < a.c.n_pages)
+          copy_rows(ring + L::VALUES, a.c.codes + (((uint64_t)id * a.c.heads + head) * 2 + 1) * KV8_PAGE * hd,
+                    sq.len - pg * (int32_t)TILE);
         copy_commit();
       };
       uint32_t id = find(tile);
@@ -352,6 +357,7 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
         const uint32_t next = find(tile + 1);
         const bool has = id < a.c.n_pages;
         copy_wait<1>();
+        __syncwarp();
         // ---- S^T = K Q^T: two tiles of 16 positions ----
         float s[NB][2][4] = {};
         if (has) {
@@ -359,7 +365,7 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
           for (int sg = 0; sg < SEG; sg++) {
             uint4 k[4];
 #pragma unroll
-            for (int n = 0; n < 4; n++) k[n] = lds16(ring + lane * 16 + (n * SEG + sg) * 512);
+            for (int n = 0; n < 4; n++) k[n] = lds16(ring + L::at(n * 8 + g, sg * 4 + t));
 #pragma unroll
             for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -375,7 +381,8 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
               }
           }
         }
-        const uint2 sc = lds8(ring + L::SCALES + lane * 8);
+        const uint2 sc = lds8(ring + L::SCALES);
+        __syncwarp();
         fetch_k(tile + 1, next);
         uint32_t pf[NB][2][SPLIT ? 4 : 2];
         if (has) {
@@ -458,6 +465,7 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
           }
         }
         copy_wait<1>();
+        __syncwarp();
         // ---- O^T += V^T P^T ----
         if (has) {
 #pragma unroll
@@ -465,11 +473,12 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
             uint32_t vr[4][HDV / 32];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
+              const uint32_t row = 16 * half + 2 * t + (i & 1) + 8 * (i >> 1);
               if constexpr (HDV == 128) {
-                const uint4 v = lds16(ring + L::VALUES + lane * 16 + (4 * half + i) * 512);
+                const uint4 v = lds16(ring + L::VALUES + L::at(row, g));
                 vr[i][0] = v.x, vr[i][1] = v.y, vr[i][2] = v.z, vr[i][3] = v.w;
               } else {
-                const uint2 v = lds8(ring + L::VALUES + lane * 8 + (4 * half + i) * 256);
+                const uint2 v = lds8(ring + L::VALUES + L::at(row, g >> 1) + (g & 1) * 8);
                 vr[i][0] = v.x, vr[i][1] = v.y;
               }
             }
@@ -493,6 +502,7 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
             }
           }
         }
+        __syncwarp();
         fetch_v(tile + 1, next);
         id = next;
       }
