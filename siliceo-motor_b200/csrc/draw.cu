@@ -8,14 +8,21 @@
 //   running sum of w passes u times the kept sum
 //
 // Which token comes out is a comparison of sums of up to 2^19 weights, so
-// weights are 64-bit fixed-point numbers (2^-43; the exponential is evaluated
-// in f64): their sums are exact, whatever the order, and the atomics of a
-// histogram cannot change a draw.
+// weights are 64-bit fixed-point numbers (2^-43, from an f64 evaluation): their
+// sums are exact, whatever the order, and atomics cannot change a draw.
 //
-// A cluster of CTAs holds a row in shared memory and reads it once. The k-th
-// largest value and the nucleus's border are found without sorting the row: a
-// histogram over the distance from the maximum, then an exact sort of the one
-// bin the border lies in (or finer histograms while that bin holds too many).
+// A cluster of CTAs holds a row in shared memory and reads it once. No row is
+// sorted: a histogram (2048 bins over the distance from the maximum) gives the
+// bin in which the k-th largest value, or the nucleus's border, lies, and only
+// that bin's values are ordered. For top-p the histogram's counts times the
+// weight at a bin's middle give a guess, which one pass over the exact weights
+// confirms (or widens). Bins that hold more than CAP values (long ties) are
+// split again over (value, index). With top_k up to about a thousand the few
+// candidates go to one CTA, which finishes the row.
+//
+// Bound by latency for one row (passes over shared memory and cluster
+// barriers), by the f64 pipe where every weight is needed (top-p, min-p and
+// plain sampling: ten operations a value).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -30,10 +37,11 @@ namespace cg = cooperative_groups;
 namespace sm {
 namespace {
 
-constexpr uint32_t THREADS = 512;
+constexpr uint32_t THREADS = 512, WARPS = THREADS / 32;
 constexpr uint32_t BINS = 2048;
-constexpr uint32_t CAP = 1024;    // candidates sorted at once
+constexpr uint32_t CAP = 1024;            // values ordered at once
 constexpr double UNIT = 8796093022208.0;  // 2^43
+constexpr double RANGE = 24.0;                // the histogram's: e^-24 of the largest weight, the last bin what is below
 constexpr uint32_t MAX_CLUSTER = 16;
 
 // Order-preserving integer of a float, and a value's place in a row's order:
@@ -49,289 +57,562 @@ __device__ __forceinline__ float load_logit(float x) { return x; }
 __device__ __forceinline__ float load_logit(__half x) { return __half2float(x); }
 __device__ __forceinline__ float load_logit(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-struct Shared {
+// What the CTAs of a cluster see of one another.
+struct alignas(16) Shared {
   uint32_t count[BINS];
-  uint64_t mass[BINS];
-  uint64_t cand[CAP];     // gathered places (rank 0's), then sorted
-  uint64_t sorted[CAP];
-  uint64_t warp64[THREADS / 32], warp64b[THREADS / 32];
-  uint64_t post[4];       // what this CTA tells the cluster
-  uint64_t got[4];        // what the cluster found
-  uint32_t n_cand;
+  uint64_t cand[CAP], sorted[CAP];  // places gathered by rank 0, and in order
+  uint64_t weight[CAP];             // of the sorted ones
+  double exp2_of[64];               // 2^(43 + j / 64)
+  uint64_t warp64[WARPS], warp64b[WARPS];
+  uint64_t post[10];                // what this CTA tells the others; no slot is written again before all have read it
+  uint64_t cut;                     // rank 0's answer
+  uint32_t n_cand, found[2];
 };
 
+static_assert(sizeof(Shared) % 16 == 0, "the values behind it are read as float4");
+
+// Sum over the CTA, in every thread. `tmp` may be reused after the next barrier.
 __device__ uint64_t block_sum(uint64_t v, uint64_t* tmp) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) tmp[threadIdx.x >> 5] = v;
   __syncthreads();
   v = 0;
-  for (uint32_t i = 0; i < THREADS / 32; i++) v += tmp[i];
+#pragma unroll
+  for (uint32_t i = 0; i < WARPS; i++) v += tmp[i];
   return v;
-}
-// Exclusive prefix of v over the CTA's threads.
-__device__ uint64_t block_before(uint64_t v, uint64_t* tmp, uint64_t* total) {
-  const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  uint64_t x = v;
-  for (uint32_t o = 1; o < 32; o <<= 1) {
-    const uint64_t y = __shfl_up_sync(~0u, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) tmp[w] = x;
-  __syncthreads();
-  uint64_t before = 0, all = 0;
-  for (uint32_t i = 0; i < THREADS / 32; i++) {
-    before += i < w ? tmp[i] : 0;
-    all += tmp[i];
-  }
-  *total = all;
-  return before + x - v;
 }
 __device__ uint64_t block_max(uint64_t v, uint64_t* tmp) {
   for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor_sync(~0u, v, o));
   __syncthreads();
   if ((threadIdx.x & 31) == 0) tmp[threadIdx.x >> 5] = v;
   __syncthreads();
-  for (uint32_t i = 0; i < THREADS / 32; i++) v = max(v, tmp[i]);
+#pragma unroll
+  for (uint32_t i = 0; i < WARPS; i++) v = max(v, tmp[i]);
   return v;
 }
+// Exclusive prefix over the CTA's threads, and the sum.
+template <typename N>
+__device__ N block_before(N v, uint64_t* tmp64, N* total) {
+  N* tmp = reinterpret_cast<N*>(tmp64);
+  const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  N x = v;
+#pragma unroll
+  for (uint32_t o = 1; o < 32; o <<= 1) {
+    const N y = __shfl_up_sync(~0u, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) tmp[w] = x;
+  __syncthreads();
+  N before = 0, all = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < WARPS; i++) {
+    before += i < w ? tmp[i] : (N)0;
+    all += tmp[i];
+  }
+  *total = all;
+  return before + (x - v);
+}
 
-struct Row {
-  const float* x;        // this CTA's values in shared memory
-  uint32_t n, begin;     // how many, and the first's index
-  uint32_t each;         // consecutive values of a thread (odd: no bank conflicts)
-  float top;             // the row's maximum
-  double inv_t;
-  __device__ double w(float v) const { return exp(((double)v - (double)top) * inv_t); }
-  __device__ uint64_t fixed(float v) const { return (uint64_t)(w(v) * UNIT + 0.5); }
+// Weights of a row: 2^43 exp((x - top) / T) = 2^(43 + y), y = (x - top) c.
+// y = k / 64 + r, |r| <= 1/128: 2^(k/64) from a table and the exponent, 2^r by
+// its Taylor polynomial of degree 4 (relative error (ln2 / 128)^5 / 120 < 2^-44).
+struct Weights {
+  const double* table;
+  double c, top;
+  // A float in f64, by its bits (zero and subnormals come out as values below 2^-126: no weight changes by it).
+  static __device__ double wide(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(b << 29));
+  }
+  __device__ uint64_t of(float x) const {
+    const double y = (wide(x) - top) * c;
+    constexpr double magic = 6755399441055744.0 / 64;  // 1.5 2^52 / 64: adding it rounds to a multiple of 1/64
+    const double t = y + magic;
+    const int k = __double2loint(t);
+    const double r = y - (t - magic);
+    constexpr double L = 0.69314718055994530942;
+    double p = fma(r, L * L * L * L / 24, L * L * L / 6);
+    p = fma(p, r, L * L / 2);
+    p = fma(p, r, L);
+    p = fma(p, r, 1.0);
+    // the product, in [2^43, 2^44) or a rounding off, as an integer: the low bits behind 2^52
+    const uint64_t v = (uint64_t)__double_as_longlong(fma(table[k & 63], p, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+    const int s = -(k >> 6) & 63;
+    return y < -44.0 ? 0 : (v + ((uint64_t)1 << s >> 1)) >> s;  // -inf gets here too
+  }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS) draw_kernel(const DrawArgs a, uint32_t chunk) {
+__global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint32_t chunk) {
   extern __shared__ float4 draw_smem4[];
   Shared& sh = *reinterpret_cast<Shared*>(draw_smem4);
   float* vals = reinterpret_cast<float*>(&sh + 1);
   cg::cluster_group cl = cg::this_cluster();
   const uint32_t CL = cl.num_blocks(), rank = cl.block_rank(), row = blockIdx.x / CL, tid = threadIdx.x;
-  const uint32_t V = a.vocab;
-  Row r;
-  r.begin = min(V, rank * chunk);
-  r.n = min(V, r.begin + chunk) - r.begin;
-  r.each = (r.n + THREADS - 1) / THREADS | 1;
-  r.x = vals;
+  const uint32_t lane = tid & 31, V = a.vocab;
+  const uint32_t begin = min(V, rank * chunk), n = min(V, begin + chunk) - begin;  // this CTA's part of the row
+  auto peer = [&](uint32_t i) { return cl.map_shared_rank(&sh, i); };
 
-  // ---- the row's part, into shared memory; its largest ----
-  uint64_t best = 0;
+  // ---- the part, into shared memory; the largest value, the lowest index among equals ----
+  float mine_x = -INFINITY;  // this thread's largest
+  uint32_t mine_i = 0;
   {
-    const T* src = (const T*)a.logits + (uint64_t)row * a.ld + r.begin;
-    const uint8_t* mk = a.mask ? a.mask + (uint64_t)row * a.ld + r.begin : nullptr;
-    for (uint32_t i = tid; i < r.n; i += THREADS) {
-      float x = load_logit(src[i]);
-      if (!(x > -INFINITY) || (mk && !mk[i])) x = -INFINITY;  // NaN, masked
-      x = fminf(x, FLT_MAX) + 0.f;                            // and -0 is 0
+    const T* src = (const T*)a.logits + (uint64_t)row * a.ld + begin;
+    const uint8_t* mk = a.mask ? a.mask + (uint64_t)row * a.ld + begin : nullptr;
+    auto take = [&](uint32_t i, float x) {
+      x = x > -INFINITY && (!mk || mk[i]) ? fminf(x, FLT_MAX) + 0.f : -INFINITY;  // NaN, masked; -0 is 0
       vals[i] = x;
-      if (x > -INFINITY) best = max(best, place(x, r.begin + i));
+      if (x > mine_x) mine_x = x, mine_i = i;
+    };
+    constexpr uint32_t PER = 16 / sizeof(T), AHEAD = 5;  // 16-byte loads, five in flight
+    const uint32_t nv = (uintptr_t)src % 16 == 0 ? n / PER : 0;
+    for (uint32_t i = tid; i < nv; i += THREADS * AHEAD) {
+      uint4 raw[AHEAD];
+#pragma unroll
+      for (uint32_t k = 0; k < AHEAD; k++)
+        if (i + k * THREADS < nv) raw[k] = __ldcs(reinterpret_cast<const uint4*>(src) + i + k * THREADS);
+#pragma unroll
+      for (uint32_t k = 0; k < AHEAD; k++)
+        if (i + k * THREADS < nv) {
+#pragma unroll
+          for (uint32_t j = 0; j < PER; j++) take((i + k * THREADS) * PER + j, load_logit(reinterpret_cast<const T*>(&raw[k])[j]));
+        }
     }
+    for (uint32_t i = nv * PER + tid; i < n; i += THREADS) take(i, load_logit(src[i]));
   }
+  uint64_t best = mine_x > -INFINITY ? place(mine_x, begin + mine_i) : 0;
+  for (uint32_t b = tid; b < BINS; b += THREADS) sh.count[b] = 0;
+  if (tid < 64) sh.exp2_of[tid] = exp2(43.0 + tid / 64.0);
   best = block_max(best, sh.warp64);
-  if (tid == 0) sh.post[0] = best, sh.n_cand = 0, sh.got[0] = 0;
-  cl.sync();
-  for (uint32_t i = 0; i < CL; i++) best = max(best, cl.map_shared_rank(&sh, i)->post[0]);
+  if (tid == 0) sh.post[0] = best, sh.n_cand = 0;
   const DrawParams p = a.params[row];
-  const bool sampled = p.temperature > 0.f;
-  if (best == 0 || !sampled) {  // nothing to draw from, or greedy
+  float u = a.u[row];
+  cl.sync();
+  {
+    uint64_t v[MAX_CLUSTER];
+#pragma unroll
+    for (uint32_t i = 0; i < MAX_CLUSTER; i++) v[i] = i < CL ? peer(i)->post[0] : 0;
+#pragma unroll
+    for (uint32_t i = 0; i < MAX_CLUSTER; i++) best = max(best, v[i]);
+  }
+  if (best == 0 || !(p.temperature > 0.f)) {  // nothing to draw from, or greedy
     if (rank == 0 && tid == 0) {
       a.tokens[row] = best ? (int32_t)(uint32_t)~best : -1;
       if (a.logprobs) a.logprobs[row] = best ? 0.f : -INFINITY;
     }
-    cl.sync();  // post is read above
+    cl.sync();  // the others read post
     return;
   }
-  r.top = unordered((uint32_t)(best >> 32));
-  r.inv_t = 1.0 / (double)p.temperature;
-  const uint32_t i0 = min(r.n, tid * r.each), i1 = min(r.n, i0 + r.each);
-  float uu = a.u[row];
-  uu = uu > 0.f ? fminf(uu, 0.99999994f) : 0.f;
-  const double min_p = p.min_p;
-  auto peer = [&](uint32_t i) { return cl.map_shared_rank(&sh, i); };
+  const float top = unordered((uint32_t)(best >> 32));
+  const double inv_t = 1.0 / (double)p.temperature;
+  Weights wt;
+  wt.table = sh.exp2_of;
+  wt.c = inv_t * 1.4426950408889634074;
+  wt.top = Weights::wide(top);
+  u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
+  // kept: weights of at least this
+  const double min_w = fmin(ceil(fmax((double)p.min_p, 0.0) * UNIT), 1e18);
+  const uint64_t min_weight = (uint64_t)min_w;
+  auto finish = [&](uint32_t index, float x, uint64_t total) {
+    a.tokens[row] = (int32_t)index;
+    if (a.logprobs) a.logprobs[row] = (float)(((double)x - (double)top) * inv_t - log((double)total / UNIT));
+  };
+  // f(x, index in this CTA's part) for this thread's share of the values, -inf among them
+  auto each = [&](auto f) {
+    const uint32_t n4 = n / 4;
+#pragma unroll 2
+    for (uint32_t i = tid; i < n4; i += THREADS) {
+      const float4 v = reinterpret_cast<const float4*>(vals)[i];
+      f(v.x, 4 * i), f(v.y, 4 * i + 1), f(v.z, 4 * i + 2), f(v.w, 4 * i + 3);
+    }
+    if (4 * n4 + tid < n) f(vals[4 * n4 + tid], 4 * n4 + tid);
+  };
+  // The cluster's bins added up: thread t has bins [4t, 4t + 4)
+  auto all_counts = [&](uint32_t (&c)[4]) {
+    for (uint32_t i0 = 0; i0 < CL; i0 += 8) {
+      uint4 v[8];
+#pragma unroll
+      for (uint32_t i = 0; i < 8; i++) v[i] = i0 + i < CL ? reinterpret_cast<const uint4*>(peer(i0 + i)->count)[tid] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (uint32_t i = 0; i < 8; i++) c[0] += v[i].x, c[1] += v[i].y, c[2] += v[i].z, c[3] += v[i].w;
+    }
+  };
+  // Orders the n values of sh.cand, largest first, into sh.sorted: by counting
+  // the larger ones while that is less work than a bitonic network.
+  auto order = [&](uint32_t count) {
+    __syncthreads();
+    if (count <= 256) {  // two threads a value
+      const uint32_t i = tid >> 1;
+      if (i < (count + 15) / 16 * 16) {
+        const uint64_t c = i < count ? sh.cand[i] : 0;
+        uint32_t before = 0;
+#pragma unroll 8
+        for (uint32_t j = tid & 1; j < count; j += 2) before += sh.cand[j] > c;
+        before += __shfl_xor_sync(~0u, before, 1);
+        if (i < count && !(tid & 1)) sh.sorted[before] = c;
+      }
+    } else {
+      uint32_t size = 512;
+      while (size < count) size *= 2;
+      for (uint32_t i = tid; i < size; i += THREADS) sh.sorted[i] = i < count ? sh.cand[i] : 0;
+      __syncthreads();
+      for (uint32_t len = 2; len <= size; len *= 2)
+        for (uint32_t step = len / 2; step; step /= 2) {
+          for (uint32_t i = tid; i < size / 2; i += THREADS) {
+            const uint32_t x = (i & ~(step - 1)) * 2 + (i & (step - 1)), y = x + step;
+            const uint64_t vx = sh.sorted[x], vy = sh.sorted[y];
+            if ((vx < vy) == ((x & len) == 0)) sh.sorted[x] = vy, sh.sorted[y] = vx;
+          }
+          // pairs up to 32 apart lie in the 64 values of one warp
+          if (step > 32 || (step == 1 && len >= 64)) __syncthreads(); else __syncwarp();
+        }
+    }
+    __syncthreads();
+  };
 
-  // One round of the search for a border among the places in [lo, hi]. By
-  // count: the border is the `goal`-th largest place. By mass: the place whose
-  // preceding mass is still below `goal` of `mass_all`, the last such. `above`
-  // is the count (or mass) of the places over hi. First round: bins over the
-  // distance from the maximum; later ones over [lo, hi] itself. Leaves in
-  // sh.got: {first place of the bin's values as the caller narrows it, bin, above, number in the bin}.
-  uint64_t cut = 0;  // places >= cut are kept
   const bool by_k = p.top_k > 0 && (uint32_t)p.top_k < V, by_p = p.top_p < 1.f;
-  const float bin_scale = (float)fmin(BINS * r.inv_t / 24.0, (double)FLT_MAX);
+  const float bin_scale = (float)fmin(BINS * inv_t / RANGE, (double)FLT_MAX);
+  // Rank 0: the nucleus, min-p and the draw among the first `kept` of sh.sorted, the row's top_k.
+  auto draw_sorted = [&](uint32_t kept) {
+    constexpr uint32_t PER = CAP / THREADS;
+    uint64_t w[PER], mine = 0, sum;
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) {
+      const uint32_t at = tid * PER + j;
+      w[j] = at < kept ? wt.of(unordered((uint32_t)(sh.sorted[at] >> 32))) : 0;
+      mine += w[j];
+    }
+    const uint64_t run0 = block_before(mine, sh.warp64, &sum);
+    uint64_t run = run0, in = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) {
+      const uint32_t at = tid * PER + j;
+      const bool keep = at < kept && (at == 0 || ((!by_p || (double)run < (double)p.top_p * (double)sum) && w[j] >= min_weight));
+      in += keep;
+      run += w[j];
+      sh.weight[at] = keep ? w[j] : 0;
+    }
+    kept = (uint32_t)block_sum(in, sh.warp64b);  // a prefix
+    uint64_t sum_kept = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) sum_kept += sh.weight[tid * PER + j];
+    sum_kept = block_sum(sum_kept, sh.warp64);
+    const double aim = (double)u * (double)sum_kept;
+    // the kept ones again, in the order of their indices
+    for (uint32_t i = tid; i < kept; i += THREADS) sh.cand[i] = (uint64_t)(uint32_t)sh.sorted[i] << 32 | i;
+    uint64_t keys[PER];
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) keys[j] = tid + j * THREADS < kept ? sh.sorted[tid + j * THREADS] >> 32 : 0;
+    order(kept);
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++)  // cand: the values, as they were sorted
+      if (tid + j * THREADS < kept) sh.cand[tid + j * THREADS] = keys[j];
+    __syncthreads();
+    mine = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) {
+      const uint32_t at = tid * PER + j;
+      w[j] = at < kept ? sh.weight[(uint32_t)sh.sorted[at]] : 0;
+      mine += w[j];
+    }
+    run = block_before(mine, sh.warp64, &sum);
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) {
+      const uint32_t at = tid * PER + j;
+      if (at < kept && (double)run <= aim && (double)(run + w[j]) > aim)
+        finish(~(uint32_t)(sh.sorted[at] >> 32), unordered((uint32_t)sh.cand[(uint32_t)sh.sorted[at]]), sum_kept);
+      run += w[j];
+    }
+  };
+  auto fast_bin = [&](float x) { return (top - x) * bin_scale; };
 
+  uint64_t cut = 0;  // places >= cut are kept
+  if (by_k && p.top_k <= (int32_t)CAP / 2) {
+    // At least top_k of the row's values reach the top_k-th largest of the threads' maxima, and few others
+    // do: a histogram of the maxima alone gives the bin down to which all values are gathered.
+    if (mine_x > -INFINITY) atomicAdd(&sh.count[(uint32_t)fminf(fast_bin(mine_x), (float)(BINS - 1))], 1u);
+    if (tid == 0) sh.found[0] = ~0u;
+    cl.sync();
+    uint32_t c[4] = {}, all;
+    all_counts(c);
+    uint32_t before = block_before(c[0] + c[1] + c[2] + c[3], sh.warp64, &all);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (before < (uint32_t)p.top_k && before + c[j] >= (uint32_t)p.top_k) sh.found[0] = 4 * tid + j;
+      before += c[j];
+    }
+    __syncthreads();
+    const uint32_t bin = sh.found[0];
+    uint32_t gathered = CAP + 1;
+    if (bin < BINS - 1) {
+      Shared* zero = peer(0);
+      const float behind = (float)(bin + 1);
+      each([&](float x, uint32_t i) {
+        if (fast_bin(x) < behind) {
+          const uint32_t at = atomicAdd(&zero->n_cand, 1u);
+          if (at < CAP) zero->cand[at] = place(x, begin + i);
+        }
+      });
+      cl.sync();
+      gathered = zero->n_cand;
+    }
+    if (gathered <= CAP) {
+      cl.sync();  // the others have read it
+      if (rank == 0) {
+        order(gathered);
+        draw_sorted(min(gathered, (uint32_t)p.top_k));
+      }
+      return;
+    }
+    cl.sync();  // the others have read the counts and n_cand
+    for (uint32_t b = tid; b < BINS; b += THREADS) sh.count[b] = 0;
+    if (tid == 0) sh.n_cand = 0;
+  }
   for (int phase = 0; phase < 2; phase++) {
-    // phase 0: top-k by counts; phase 1: top-p by mass among the places >= cut
+    // phase 0: the top_k-th place, by counts; phase 1: the nucleus's border, by mass among the places >= cut
     if (phase == 0 ? !by_k : !by_p) continue;
     const bool mass = phase == 1;
-    uint64_t lo = cut, hi = best, above = 0, all = 0;
+    uint64_t lo = cut, hi = best, above = 0;  // the border lies in [lo, hi]; count or mass over hi
+    double goal = 0;
+    uint32_t slot = 1;
+    if (mass && by_k) {
+      cl.sync();  // the others have read the counts of phase 0
+      for (uint32_t b = tid; b < BINS; b += THREADS) sh.count[b] = 0;
+    }
     for (int round = 0;; round++) {
-      int sh_bits = 0;
-      if (round) while (((hi - lo) >> sh_bits) >= BINS) sh_bits++;
+      int bits = 0;
+      if (round) while (((hi - lo) >> bits) >= BINS) bits++;
       auto bin_of = [&](float x, uint64_t pl) -> uint32_t {
-        return round ? (uint32_t)((hi - pl) >> sh_bits) : min(BINS - 1, (uint32_t)fminf((r.top - x) * bin_scale, 4e9f));
+        return round ? (uint32_t)((hi - pl) >> bits) : (uint32_t)fminf(fast_bin(x), (float)(BINS - 1));
       };
-      for (uint32_t b = tid; b < BINS; b += THREADS) sh.count[b] = 0, sh.mass[b] = 0;
+      const bool everything = round == 0 && lo == 0;  // every value is in [lo, hi]: only its bin matters
       __syncthreads();
-      for (uint32_t i = i0; i < i1; i++) {
-        const float x = vals[i];
-        const uint64_t pl = place(x, r.begin + i);
-        if (x == -INFINITY || pl < lo || pl > hi) continue;
-        const uint32_t b = bin_of(x, pl);
-        atomicAdd(&sh.count[b], 1u);
-        if (mass) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[b]), (unsigned long long)r.fixed(x));
+      if (everything) {
+        each([&](float x, uint32_t) {
+          if (x > -INFINITY) atomicAdd(&sh.count[(uint32_t)fminf(fast_bin(x), (float)(BINS - 1))], 1u);
+        });
+      } else {
+        each([&](float x, uint32_t i) {
+          const uint64_t pl = place(x, begin + i);
+          if (x > -INFINITY && pl >= lo && pl <= hi) atomicAdd(&sh.count[bin_of(x, pl)], 1u);
+        });
       }
       cl.sync();
-      // this CTA adds up the cluster's bins [b0, b0 + per)
-      const uint32_t per = BINS / CL, b0 = rank * per;
-      uint64_t c_mine = 0, m_mine = 0;  // of this thread's bins: consecutive ones
-      const uint32_t tper = (per + THREADS - 1) / THREADS, t0 = min(per, tid * tper), t1 = min(per, t0 + tper);
-      uint64_t cs[4] = {}, ms[4] = {};  // BINS / THREADS at most
-      for (uint32_t b = t0; b < t1; b++) {
-        for (uint32_t i = 0; i < CL; i++) {
-          cs[b - t0] += peer(i)->count[b0 + b];
-          if (mass) ms[b - t0] += peer(i)->mass[b0 + b];
+      uint32_t c[4] = {};
+      all_counts(c);
+      uint32_t c_total;
+      const uint32_t c_before = block_before(c[0] + c[1] + c[2] + c[3], sh.warp64, &c_total);
+      uint32_t bin_a = 0, bin_b = BINS - 1;  // the border lies in a bin from bin_a to bin_b
+      uint64_t mass_above = 0;               // of the bins before bin_a
+      uint64_t n_above, n_in;                // places in the bins before, and in them
+      auto count_range = [&] {
+        uint64_t ca = 0, ci = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint32_t b = 4 * tid + j;
+          ca += b < bin_a ? c[j] : 0;
+          ci += b >= bin_a && b <= bin_b ? c[j] : 0;
         }
-        c_mine += cs[b - t0], m_mine += ms[b - t0];
-      }
-      uint64_t c_total, m_total;
-      const uint64_t c_before = block_before(c_mine, sh.warp64, &c_total);
-      const uint64_t m_before = block_before(m_mine, sh.warp64b, &m_total);
-      if (tid == 0) sh.post[1] = c_total, sh.post[2] = m_total;
-      cl.sync();
-      uint64_t c_run = mass ? 0 : above, m_run = above, m_all = 0;
-      for (uint32_t i = 0; i < CL; i++) {
-        if (i < rank) c_run += peer(i)->post[1], m_run += peer(i)->post[2];
-        m_all += peer(i)->post[2];
-      }
-      if (mass && !round) all = m_all;
-      c_run += c_before, m_run += m_before;
-      const double goal = (double)p.top_p * (double)all;
-      // the bin with the border: the last whose values begin before the goal
-      for (uint32_t b = t0; b < t1; b++) {
-        const uint64_t c = cs[b - t0], m = ms[b - t0];
-        const bool here = c && (mass ? m_run == 0 || (double)m_run < goal : c_run < (uint64_t)p.top_k);
-        const bool next = mass ? (double)(m_run + m) < goal : c_run + c < (uint64_t)p.top_k;
-        // the goal lies in this bin, or behind all of them
-        if (here && !next)
-          for (uint32_t i = 0; i < CL; i++) {
-            peer(i)->got[0] = 1, peer(i)->got[1] = b0 + b;
-            peer(i)->got[2] = mass ? m_run : c_run, peer(i)->got[3] = c;
-          }
-        c_run += c, m_run += m;
-      }
-      cl.sync();
-      const bool found = sh.got[0];
-      const uint32_t bin = (uint32_t)sh.got[1];
-      const uint64_t found_above = sh.got[2];
-      const uint32_t n_in = (uint32_t)sh.got[3];
+        const uint64_t both = block_sum(ca << 32 | ci, sh.warp64);
+        n_above = both >> 32, n_in = (uint32_t)both;
+      };
+      if (tid == 0) sh.found[0] = ~0u, sh.found[1] = ~0u;
       __syncthreads();
-      if (tid == 0) sh.got[0] = 0;
-      if (!found) break;  // fewer values than top_k, or a top_p their sum does not reach: all are kept
-      above = found_above;
+      if (!mass) {
+        uint64_t run = above + c_before;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (run < (uint64_t)p.top_k && run + c[j] >= (uint64_t)p.top_k) sh.found[0] = 4 * tid + j;
+          run += c[j];
+        }
+        __syncthreads();
+        bin_a = bin_b = sh.found[0];
+        if (bin_a == ~0u) break;  // fewer places than top_k: all are kept
+        count_range();
+      } else {
+        // The guess: counts times the weight at a bin's middle, within a margin.
+        double m[4], sum = 0, all;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint64_t b = 4 * tid + j;
+          const uint64_t mid = hi - min(hi - lo, (b << bits) + ((uint64_t)1 << bits) / 2);
+          const float y = round ? (unordered((uint32_t)(mid >> 32)) - top) * (float)wt.c
+                                : -((float)b + 0.5f) * (float)(RANGE / BINS * 1.4426950408889634);
+          m[j] = c[j] ? (double)c[j] * (double)exp2f(y) : 0.0;
+          sum += m[j];
+        }
+        double run = block_before(sum, sh.warp64b, &all);
+        const double want = round ? (goal - (double)above) / UNIT : (double)p.top_p * all, slack = 1e-3 * all;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (run < want - slack && run + m[j] >= want - slack) sh.found[0] = 4 * tid + j;
+          if (run < want + slack && run + m[j] >= want + slack) sh.found[1] = 4 * tid + j;
+          run += m[j];
+        }
+        __syncthreads();
+        // Exact masses of a range to try; it then holds the border, or what lies on one side of it does.
+        // The first is the guess, later ones halves: the range shrinks every turn.
+        uint32_t try_a = sh.found[0] == ~0u ? 0 : sh.found[0], try_b = sh.found[1] == ~0u ? BINS - 1 : max(sh.found[1], try_a);
+        for (int turn = 0;; turn++) {
+          uint64_t ma = 0, mi = 0, ml = 0;
+          if (everything && !turn) {
+            const float fa = (float)try_a, fb = try_b == BINS - 1 ? INFINITY : (float)(try_b + 1);
+            each([&](float x, uint32_t) {
+              const float b = fast_bin(x);
+              const uint64_t w = wt.of(x);
+              ma += b < fa ? w : 0;
+              mi += b >= fa && b < fb ? w : 0;
+              ml += b >= fb ? w : 0;
+            });
+          } else {
+            each([&](float x, uint32_t i) {
+              const uint64_t pl = place(x, begin + i);
+              if (!(x > -INFINITY) || pl < lo || pl > hi) return;
+              const uint32_t b = bin_of(x, pl);
+              if ((round || turn) && b > try_b) return;
+              const uint64_t w = wt.of(x);
+              ma += b < try_a ? w : 0;
+              mi += b >= try_a && b <= try_b ? w : 0;
+              ml += b > try_b ? w : 0;
+            });
+          }
+          ma = block_sum(ma, sh.warp64);
+          mi = block_sum(mi, sh.warp64b);
+          ml = block_sum(ml, sh.warp64);
+          slot ^= 5;  // 1 and 4 in turn
+          if (tid == 0) sh.post[slot] = ma, sh.post[slot + 1] = mi, sh.post[slot + 2] = ml;
+          cl.sync();
+          ma = mi = ml = 0;
+#pragma unroll 8
+          for (uint32_t i = 0; i < CL; i++) ma += peer(i)->post[slot], mi += peer(i)->post[slot + 1], ml += peer(i)->post[slot + 2];
+          if (!round && !turn) goal = (double)p.top_p * (double)(ma + mi + ml);
+          const bool begins = try_a == bin_a || above + ma == 0 || (double)(above + ma) < goal;
+          const bool ends = try_b == bin_b || (double)(above + ma + mi) >= goal;
+          if (begins && ends) bin_a = try_a, bin_b = try_b, mass_above = ma;
+          else if (!begins) bin_b = try_a - 1;
+          else bin_a = try_b + 1, mass_above = ma + mi;
+          count_range();
+          if (n_in <= CAP || bin_a == bin_b) break;
+          try_a = bin_a, try_b = (bin_a + bin_b) / 2;
+        }
+      }
+      const bool small = !mass && round == 0 && n_above + n_in <= CAP;  // all the top_k at once
+      if (small) {
+        bin_a = 0;
+        n_in += n_above, n_above = 0;
+      }
       if (n_in <= CAP) {
         Shared* zero = peer(0);
-        for (uint32_t i = i0; i < i1; i++) {
-          const float x = vals[i];
-          const uint64_t pl = place(x, r.begin + i);
-          if (x == -INFINITY || pl < lo || pl > hi || bin_of(x, pl) != bin) continue;
-          zero->cand[atomicAdd(&zero->n_cand, 1u)] = pl;
-        }
+        const float fa = (float)bin_a, fb = bin_b == BINS - 1 ? INFINITY : (float)(bin_b + 1);
+        each([&](float x, uint32_t i) {
+          if (everything && !(fast_bin(x) >= fa && fast_bin(x) < fb)) return;
+          const uint64_t pl = place(x, begin + i);
+          if (!(x > -INFINITY) || pl < lo || pl > hi) return;
+          const uint32_t b = bin_of(x, pl);
+          if (b >= bin_a && b <= bin_b) zero->cand[atomicAdd(&zero->n_cand, 1u)] = pl;
+        });
         cl.sync();
+        if (small && rank != 0) return;
         if (rank == 0) {
-          for (uint32_t i = tid; i < n_in; i += THREADS) {  // rank each, by counting
-            const uint64_t c = sh.cand[i];
-            uint32_t before = 0;
-            for (uint32_t j = 0; j < n_in; j++) before += sh.cand[j] > c;
-            sh.sorted[before] = c;
-          }
-          if (tid == 0) sh.n_cand = 0;
-          __syncthreads();
-          uint64_t border = 0;
-          if (!mass) {
-            border = sh.sorted[p.top_k - 1 - above];
-          } else {
-            uint64_t mine = 0, total;
-            const uint32_t j0 = tid * (CAP / THREADS), j1 = min(n_in, j0 + CAP / THREADS);
-            for (uint32_t j = j0; j < j1; j++) mine += r.fixed(unordered((uint32_t)(sh.sorted[j] >> 32)));
-            uint64_t run = above + block_before(mine, sh.warp64, &total);
-            uint64_t keep = ~0ull;  // the smallest place whose preceding mass is below the goal
-            for (uint32_t j = j0; j < j1; j++) {
-              if (run == 0 || (double)run < goal) keep = sh.sorted[j];
-              run += r.fixed(unordered((uint32_t)(sh.sorted[j] >> 32)));
+          order((uint32_t)n_in);
+          uint32_t kept = (uint32_t)n_in;
+          if (!mass) kept = (uint32_t)((uint64_t)p.top_k - above - n_above);
+          constexpr uint32_t PER = CAP / THREADS;
+          uint64_t w[PER], mine = 0, nothing;
+          if (mass) {
+#pragma unroll
+            for (uint32_t j = 0; j < PER; j++) {
+              const uint32_t at = tid * PER + j;
+              w[j] = at < kept ? wt.of(unordered((uint32_t)(sh.sorted[at] >> 32))) : 0;
+              mine += w[j];
             }
-            border = ~block_max(~keep, sh.warp64);
           }
-          __syncthreads();
-          if (tid < CL) peer(tid)->got[1] = border;
+          if (small) {
+            draw_sorted(kept);
+            return;
+          }
+          if (mass) {
+            uint64_t run = above + mass_above + block_before(mine, sh.warp64, &nothing), in = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < PER; j++) {
+              const uint32_t at = tid * PER + j;
+              in += at < kept && ((double)run < goal || n_above + at == 0);
+              run += w[j];
+            }
+            kept = (uint32_t)block_sum(in, sh.warp64b);  // at least one: the range begins before the goal
+          }
+          if (tid == 0) sh.cut = sh.sorted[kept - 1], sh.n_cand = 0;
         }
         cl.sync();
-        cut = sh.got[1];
+        cut = peer(0)->cut;
         break;
       }
-      // too many in the bin: narrow [lo, hi] to what it holds
+      // too many: narrow [lo, hi] to what the range holds
       uint64_t mn = ~0ull, mx = 0;
-      for (uint32_t i = i0; i < i1; i++) {
-        const float x = vals[i];
-        const uint64_t pl = place(x, r.begin + i);
-        if (x == -INFINITY || pl < lo || pl > hi || bin_of(x, pl) != bin) continue;
-        mn = min(mn, pl), mx = max(mx, pl);
-      }
+      each([&](float x, uint32_t i) {
+        const uint64_t pl = place(x, begin + i);
+        if (!(x > -INFINITY) || pl < lo || pl > hi) return;
+        const uint32_t b = bin_of(x, pl);
+        if (b >= bin_a && b <= bin_b) mn = min(mn, pl), mx = max(mx, pl);
+      });
       mx = block_max(mx, sh.warp64);
       mn = ~block_max(~mn, sh.warp64b);
-      if (tid == 0) sh.post[1] = mn, sh.post[2] = mx;
+      cl.sync();  // the others have read counts and post
+      for (uint32_t b = tid; b < BINS; b += THREADS) sh.count[b] = 0;
+      if (tid == 0) sh.post[7] = mn, sh.post[8] = mx;
       cl.sync();
-      for (uint32_t i = 0; i < CL; i++) mn = min(mn, peer(i)->post[1]), mx = max(mx, peer(i)->post[2]);
+      for (uint32_t i = 0; i < CL; i++) mn = min(mn, peer(i)->post[7]), mx = max(mx, peer(i)->post[8]);
       lo = mn, hi = mx;
-      cl.sync();
+      above += mass ? mass_above : n_above;
     }
   }
 
-  // ---- the draw, in the vocabulary's order ----
-  auto kept = [&](float x, uint32_t i, double w) {
-    const uint64_t pl = place(x, i);
-    return x > -INFINITY && pl >= cut && (w >= min_p || pl == best);
+  // ---- the draw, in the vocabulary's order: a thread has consecutive values, an odd number (no bank conflicts) ----
+  const uint32_t run_len = (n + THREADS - 1) / THREADS | 1, i0 = min(n, tid * run_len), i1 = min(n, i0 + run_len);
+  const float cut_x = cut ? unordered((uint32_t)(cut >> 32)) : -INFINITY;
+  const uint32_t cut_i = ~(uint32_t)cut - begin, best_i = ~(uint32_t)best - begin;  // modulo 2^32, as begin + i is
+  auto weight_at = [&](uint32_t i) -> uint64_t {  // 0: not kept
+    const float x = vals[i];
+    const uint64_t w = wt.of(x);
+    const bool in = x > cut_x || (x == cut_x && begin + i <= cut_i + begin);
+    return in && (w >= min_weight || i == best_i) ? w : 0;
   };
   uint64_t mine = 0;
-  for (uint32_t i = i0; i < i1; i++) {
-    const float x = vals[i];
-    if (x == -INFINITY || place(x, r.begin + i) < cut) continue;
-    const double w = r.w(x);
-    if (kept(x, r.begin + i, w)) mine += (uint64_t)(w * UNIT + 0.5);
-  }
-  uint64_t cta_total;
-  const uint64_t before = block_before(mine, sh.warp64, &cta_total);
-  if (tid == 0) sh.post[3] = cta_total;
+#pragma unroll 4
+  for (uint32_t i = i0; i < i1; i++) mine += weight_at(i);
+  uint64_t cta;
+  uint64_t run = block_before(mine, sh.warp64, &cta);
+  if (tid == 0) sh.post[9] = cta;
   cl.sync();
-  uint64_t run = before, total = 0;
+  uint64_t total = 0;
   for (uint32_t i = 0; i < CL; i++) {
-    const uint64_t m = peer(i)->post[3];
-    if (i < rank) run += m;
+    const uint64_t m = peer(i)->post[9];
+    run += i < rank ? m : 0;
     total += m;
   }
-  const double goal = (double)uu * (double)total;
-  // one thread of the cluster holds the value at which the sum passes the goal
-  if (mine && (double)run <= goal && (double)(run + mine) > goal) {
-    for (uint32_t i = i0; i < i1; i++) {
-      const float x = vals[i];
-      if (x == -INFINITY || place(x, r.begin + i) < cut) continue;
-      const double w = r.w(x);
-      if (!kept(x, r.begin + i, w)) continue;
-      const uint64_t f = (uint64_t)(w * UNIT + 0.5);
-      if ((double)run <= goal && (double)(run + f) > goal) {
-        a.tokens[row] = (int32_t)(r.begin + i);
-        if (a.logprobs) a.logprobs[row] = (float)(((double)x - (double)r.top) * r.inv_t - log((double)total / UNIT));
+  cl.sync();  // the others read post
+  const double aim = (double)u * (double)total;
+  // one thread of the cluster holds the value at which the sum passes the aim; its warp looks for it
+  const uint32_t who = __ballot_sync(~0u, (double)run <= aim && (double)(run + mine) > aim);
+  if (who) {
+    const uint32_t owner = __ffs(who) - 1;
+    run = __shfl_sync(~0u, run, owner);
+    const uint32_t j0 = __shfl_sync(~0u, i0, owner), j1 = __shfl_sync(~0u, i1, owner);
+    for (uint32_t i = j0; i < j1; i += 32) {
+      const uint64_t w = i + lane < j1 ? weight_at(i + lane) : 0;
+      uint64_t upto = w;
+#pragma unroll
+      for (uint32_t o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += y;
       }
-      run += f;
+      upto += run;
+      if (w && (double)upto > aim && (double)(upto - w) <= aim) finish(begin + i + lane, vals[i + lane], total);
+      run = __shfl_sync(~0u, upto, 31);
     }
   }
-  cl.sync();  // post is read above
 }
 
 template <typename T>
