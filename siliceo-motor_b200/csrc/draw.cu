@@ -22,7 +22,7 @@
 //
 // Bound by latency for one row (passes over shared memory and cluster
 // barriers), by the f64 pipe where every weight is needed (top-p, min-p and
-// plain sampling: ten operations a value).
+// plain sampling: eleven operations a value).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -43,6 +43,7 @@ constexpr uint32_t CAP = 1024;            // values ordered at once
 constexpr double UNIT = 8796093022208.0;  // 2^43
 constexpr double RANGE = 24.0;                // the histogram's: e^-24 of the largest weight, the last bin what is below
 constexpr uint32_t MAX_CLUSTER = 16;
+constexpr uint32_t MAX_PART = 78 * 1024;     // bytes of a row a CTA keeps: two fit an SM
 
 // Order-preserving integer of a float, and a value's place in a row's order:
 // larger = earlier (larger value, then lower index).
@@ -56,17 +57,23 @@ __device__ __forceinline__ uint64_t place(float x, uint32_t i) { return (uint64_
 __device__ __forceinline__ float load_logit(float x) { return x; }
 __device__ __forceinline__ float load_logit(__half x) { return __half2float(x); }
 __device__ __forceinline__ float load_logit(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void store_logit(float x, float& o) { o = x; }
+__device__ __forceinline__ void store_logit(float x, __half& o) { o = __float2half_rn(x); }
+__device__ __forceinline__ void store_logit(float x, __nv_bfloat16& o) { o = __float2bfloat16_rn(x); }
+template <typename T>
+__device__ __forceinline__ float value(T x) { return fminf(load_logit(x), FLT_MAX); }  // +inf: the largest float
 
 // What the CTAs of a cluster see of one another.
 struct alignas(16) Shared {
   uint32_t count[BINS];
   uint64_t cand[CAP], sorted[CAP];  // places gathered by rank 0, and in order
   uint64_t weight[CAP];             // of the sorted ones
-  double exp2_of[64];               // 2^(43 + j / 64)
+  double exp2_of[16];               // 2^(43 + j / 16)
   uint64_t warp64[WARPS], warp64b[WARPS];
   uint64_t post[10];                // what this CTA tells the others; no slot is written again before all have read it
   uint64_t cut;                     // rank 0's answer
-  uint32_t n_cand, found[2];
+  uint64_t found_run;
+  uint32_t n_cand, found[2], n_here, n_left, at_zero;
 };
 
 static_assert(sizeof(Shared) % 16 == 0, "the values behind it are read as float4");
@@ -115,32 +122,36 @@ __device__ N block_before(N v, uint64_t* tmp64, N* total) {
   return before + (x - v);
 }
 
-// Weights of a row: 2^43 exp((x - top) / T) = 2^(43 + y), y = (x - top) c.
-// y = k / 64 + r, |r| <= 1/128: 2^(k/64) from a table and the exponent, 2^r by
-// its Taylor polynomial of degree 4 (relative error (ln2 / 128)^5 / 120 < 2^-44).
+// Weights of a row: 2^43 exp((x - top) / T) = 2^(43 + y), y = (x - top) c, as integers.
+// y = k / 16 + r, |r| <= 1/32: 2^(k/16) from a table and the exponent, 2^r by
+// its Taylor polynomial of degree 5 (relative error (ln2 / 32)^6 / 720 < 2^-42).
+// Sixteen doubles lie in different banks: no lookup conflicts.
 struct Weights {
-  const double* table;
+  const double* table;  // 2^(43 + j / 16)
   double c, top;
+  float floor;  // values below it weigh nothing
   // A float in f64, by its bits (zero and subnormals come out as values below 2^-126: no weight changes by it).
   static __device__ double wide(float x) {
     const uint32_t b = __float_as_uint(x);
     return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(b << 29));
   }
   __device__ uint64_t of(float x) const {
-    const double y = (wide(x) - top) * c;
-    constexpr double magic = 6755399441055744.0 / 64;  // 1.5 2^52 / 64: adding it rounds to a multiple of 1/64
+    const double y = (wide(fmaxf(x, floor)) - top) * c;
+    constexpr double magic = 6755399441055744.0 / 16;  // 1.5 2^52 / 16: adding it rounds to a multiple of 1/16
     const double t = y + magic;
     const int k = __double2loint(t);
     const double r = y - (t - magic);
     constexpr double L = 0.69314718055994530942;
-    double p = fma(r, L * L * L * L / 24, L * L * L / 6);
+    double p = fma(r, L * L * L * L * L / 120, L * L * L * L / 24);
+    p = fma(p, r, L * L * L / 6);
     p = fma(p, r, L * L / 2);
     p = fma(p, r, L);
     p = fma(p, r, 1.0);
-    // the product, in [2^43, 2^44) or a rounding off, as an integer: the low bits behind 2^52
-    const uint64_t v = (uint64_t)__double_as_longlong(fma(table[k & 63], p, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
-    const int s = -(k >> 6) & 63;
-    return y < -44.0 ? 0 : (v + ((uint64_t)1 << s >> 1)) >> s;  // -inf gets here too
+    const double f = table[k & 15];
+    const double scaled = __hiloint2double(__double2hiint(f) + (k >> 4 << 20), __double2loint(f));
+    // adding 2^52 rounds to a whole number and leaves it in the low bits
+    const uint64_t w = (uint64_t)__double_as_longlong(fma(scaled, p, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+    return x >= floor ? w : 0;
   }
 };
 
@@ -148,7 +159,7 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint32_t chunk) {
   extern __shared__ float4 draw_smem4[];
   Shared& sh = *reinterpret_cast<Shared*>(draw_smem4);
-  float* vals = reinterpret_cast<float*>(&sh + 1);
+  T* vals = reinterpret_cast<T*>(&sh + 1);  // as they came (16-bit ones take half the room), the masked ones -inf
   cg::cluster_group cl = cg::this_cluster();
   const uint32_t CL = cl.num_blocks(), rank = cl.block_rank(), row = blockIdx.x / CL, tid = threadIdx.x;
   const uint32_t lane = tid & 31, V = a.vocab;
@@ -162,8 +173,9 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
     const T* src = (const T*)a.logits + (uint64_t)row * a.ld + begin;
     const uint8_t* mk = a.mask ? a.mask + (uint64_t)row * a.ld + begin : nullptr;
     auto take = [&](uint32_t i, float x) {
-      x = x > -INFINITY && (!mk || mk[i]) ? fminf(x, FLT_MAX) + 0.f : -INFINITY;  // NaN, masked; -0 is 0
-      vals[i] = x;
+      x = x > -INFINITY && (!mk || mk[i]) ? x + 0.f : -INFINITY;  // NaN, masked; -0 is 0
+      store_logit(x, vals[i]);
+      x = fminf(x, FLT_MAX);  // as `value` reads it
       if (x > mine_x) mine_x = x, mine_i = i;
     };
     constexpr uint32_t PER = 16 / sizeof(T), AHEAD = 5;  // 16-byte loads, five in flight
@@ -184,19 +196,14 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
   }
   uint64_t best = mine_x > -INFINITY ? place(mine_x, begin + mine_i) : 0;
   for (uint32_t b = tid; b < BINS; b += THREADS) sh.count[b] = 0;
-  if (tid < 64) sh.exp2_of[tid] = exp2(43.0 + tid / 64.0);
+  if (tid < 16) sh.exp2_of[tid] = exp2(43.0 + tid / 16.0);
   best = block_max(best, sh.warp64);
   if (tid == 0) sh.post[0] = best, sh.n_cand = 0;
   const DrawParams p = a.params[row];
   float u = a.u[row];
   cl.sync();
-  {
-    uint64_t v[MAX_CLUSTER];
-#pragma unroll
-    for (uint32_t i = 0; i < MAX_CLUSTER; i++) v[i] = i < CL ? peer(i)->post[0] : 0;
-#pragma unroll
-    for (uint32_t i = 0; i < MAX_CLUSTER; i++) best = max(best, v[i]);
-  }
+  best = lane < CL ? peer(lane)->post[0] : 0;  // lane i asks CTA i
+  for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
   if (best == 0 || !(p.temperature > 0.f)) {  // nothing to draw from, or greedy
     if (rank == 0 && tid == 0) {
       a.tokens[row] = best ? (int32_t)(uint32_t)~best : -1;
@@ -211,6 +218,7 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
   wt.table = sh.exp2_of;
   wt.c = inv_t * 1.4426950408889634074;
   wt.top = Weights::wide(top);
+  wt.floor = (float)fmax((double)top - 60.0 / wt.c, -(double)FLT_MAX);  // 2^-60 of the largest
   u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
   // kept: weights of at least this
   const double min_w = fmin(ceil(fmax((double)p.min_p, 0.0) * UNIT), 1e18);
@@ -219,25 +227,72 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
     a.tokens[row] = (int32_t)index;
     if (a.logprobs) a.logprobs[row] = (float)(((double)x - (double)top) * inv_t - log((double)total / UNIT));
   };
+  // Where order counts a thread has consecutive values, an odd number of them (no bank conflicts).
+  const uint32_t run_len = (n + THREADS - 1) / THREADS | 1, i0 = min(n, tid * run_len), i1 = min(n, i0 + run_len);
   // f(x, index in this CTA's part) for this thread's share of the values, -inf among them
   auto each = [&](auto f) {
     const uint32_t n4 = n / 4;
 #pragma unroll 2
     for (uint32_t i = tid; i < n4; i += THREADS) {
-      const float4 v = reinterpret_cast<const float4*>(vals)[i];
-      f(v.x, 4 * i), f(v.y, 4 * i + 1), f(v.z, 4 * i + 2), f(v.w, 4 * i + 3);
+      struct alignas(4 * sizeof(T)) Four { T x[4]; };
+      const Four v = reinterpret_cast<const Four*>(vals)[i];
+#pragma unroll
+      for (int j = 0; j < 4; j++) f(value(v.x[j]), 4 * i + j);
     }
-    if (4 * n4 + tid < n) f(vals[4 * n4 + tid], 4 * n4 + tid);
+    if (4 * n4 + tid < n) f(value(vals[4 * n4 + tid]), 4 * n4 + tid);
   };
-  // The cluster's bins added up: thread t has bins [4t, 4t + 4)
+  // This CTA's sh.n_here places go behind those that rank 0's sh.cand holds; more than CAP are counted only.
+  auto push = [&](const uint64_t* from) {
+    __syncthreads();
+    const uint32_t here = sh.n_here;
+    Shared* zero = peer(0);
+    if (tid == 0) sh.at_zero = here ? atomicAdd(&zero->n_cand, here) : 0;
+    __syncthreads();
+    const uint32_t base = sh.at_zero;
+    for (uint32_t i = tid; i < min(here, CAP) && base + i < CAP; i += THREADS) zero->cand[base + i] = from[i];
+  };
+  // Rank 0's sh.cand and sh.n_cand get the places of the values that `in` picks, in any order: collected here
+  // first (in sh.sorted), so that a CTA reserves its room at rank 0 once.
+  auto gather = [&](auto in) {
+    if (tid == 0) sh.n_here = 0;
+    __syncthreads();
+    each([&](float x, uint32_t i) {
+      if (in(x, i)) {
+        const uint32_t at = atomicAdd(&sh.n_here, 1u);
+        if (at < CAP) sh.sorted[at] = place(x, begin + i);
+      }
+    });
+    push(sh.sorted);
+  };
+  // The cluster's bins added up: thread t has bins [4t, 4t + 4). A CTA adds up a slice (its threads share
+  // out the CTAs and four bins each) and gives it to all (sh.sorted).
   auto all_counts = [&](uint32_t (&c)[4]) {
-    for (uint32_t i0 = 0; i0 < CL; i0 += 8) {
-      uint4 v[8];
-#pragma unroll
-      for (uint32_t i = 0; i < 8; i++) v[i] = i0 + i < CL ? reinterpret_cast<const uint4*>(peer(i0 + i)->count)[tid] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (uint32_t i = 0; i < 8; i++) c[0] += v[i].x, c[1] += v[i].y, c[2] += v[i].z, c[3] += v[i].w;
+    static_assert(BINS == 4 * THREADS && BINS * 4 == CAP * 8, "four bins a thread");
+    const uint32_t per = THREADS / CL, from = tid / per, q = tid % per;
+    uint4* part = reinterpret_cast<uint4*>(sh.weight);
+    part[tid] = reinterpret_cast<const uint4*>(peer(from)->count)[rank * per + q];
+    __syncthreads();
+    uint4 v = make_uint4(0, 0, 0, 0);
+    for (uint32_t i = 0; i < CL; i++) {
+      const uint4 x = part[i * per + q];
+      v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
     }
+    reinterpret_cast<uint4*>(peer(from)->sorted)[rank * per + q] = v;
+    cl.sync();
+    v = reinterpret_cast<const uint4*>(sh.sorted)[tid];
+    c[0] = v.x, c[1] = v.y, c[2] = v.z, c[3] = v.w;
+    __syncthreads();
+  };
+  // All CTAs' post[slot] added up (lane i asks CTA i); `before`: those of the CTAs before this one.
+  auto add_up = [&](uint32_t slot, uint64_t& before) -> uint64_t {
+    uint64_t v = lane < CL ? peer(lane)->post[slot] : 0;
+    before = lane < rank ? v : 0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      v += __shfl_xor_sync(~0u, v, o);
+      before += __shfl_xor_sync(~0u, before, o);
+    }
+    return v;
   };
   // Orders the n values of sh.cand, largest first, into sh.sorted: by counting
   // the larger ones while that is less work than a bitonic network.
@@ -327,8 +382,61 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
     }
   };
   auto fast_bin = [&](float x) { return (top - x) * bin_scale; };
+  // Rank 0: of the `count` places in sh.cand the last, in order, before which less than `goal` lies (`run` in
+  // the places before all of them): weights, or numbers of places. Bins over the candidates' own range leave
+  // few of them; those are put in order.
+  auto border_among = [&](uint32_t count, bool mass, uint64_t run, double goal) -> uint64_t {
+    auto amount = [&](uint64_t pl) -> uint64_t { return mass ? wt.of(unordered((uint32_t)(pl >> 32))) : 1; };
+    uint64_t* bins = sh.sorted;  // and sh.weight behind it
+    static_assert(BINS == 2 * CAP && CAP == 2 * THREADS, "two candidates and four bins a thread");
+    while (count > 256) {
+      uint64_t pl[2];
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 2; j++) pl[j] = tid + j * THREADS < count ? sh.cand[tid + j * THREADS] : 0;
+      const uint64_t hi = block_max(max(pl[0], pl[1]), sh.warp64);
+      const uint64_t lo = ~block_max(max(pl[0] ? ~pl[0] : 0, pl[1] ? ~pl[1] : 0), sh.warp64b);
+      const int bits = max(0, 53 - __clzll(hi - lo));  // (hi - lo) >> bits is below BINS, its half or more if bits > 0
+#pragma unroll
+      for (int j = 0; j < 4; j++) bins[tid + j * THREADS] = 0;
+      if (tid == 0) sh.found[0] = 0, sh.n_left = 0;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+        if (pl[j]) atomicAdd(reinterpret_cast<unsigned long long*>(&bins[(hi - pl[j]) >> bits]), (unsigned long long)amount(pl[j]));
+      __syncthreads();
+      uint64_t m[4], sum = 0, all;
+#pragma unroll
+      for (int j = 0; j < 4; j++) m[j] = bins[4 * tid + j], sum += m[j];
+      uint64_t at = run + block_before(sum, sh.warp64, &all);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (m[j] && (at == 0 || (double)at < goal) && !((double)(at + m[j]) < goal)) sh.found[0] = 4 * tid + j, sh.found_run = at;
+        at += m[j];
+      }
+      __syncthreads();
+      const uint32_t bin = sh.found[0];
+      run = sh.found_run;
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+        if (pl[j] && (uint32_t)((hi - pl[j]) >> bits) == bin) sh.cand[atomicAdd(&sh.n_left, 1u)] = pl[j];
+      __syncthreads();
+      count = sh.n_left;
+    }
+    order(count);
+    const uint64_t own = tid < count ? amount(sh.sorted[tid]) : 0;
+    uint64_t all;
+    const uint64_t at = run + block_before(own, sh.warp64, &all);
+    const uint64_t kept = block_sum(tid < count && (tid == 0 || (double)at < goal), sh.warp64b);  // a prefix
+    return sh.sorted[kept - 1];
+  };
 
   uint64_t cut = 0;  // places >= cut are kept
+  // The nucleus's border lay in a range of at most CAP places, which each CTA has in `local` (the bins are
+  // done with then), and `mine` is the mass of this thread's consecutive values before that range.
+  bool direct = false;
+  uint64_t mine = 0;
+  uint64_t* local = reinterpret_cast<uint64_t*>(sh.count);
   if (by_k && p.top_k <= (int32_t)CAP / 2) {
     // At least top_k of the row's values reach the top_k-th largest of the threads' maxima, and few others
     // do: a histogram of the maxima alone gives the bin down to which all values are gathered.
@@ -347,16 +455,10 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
     const uint32_t bin = sh.found[0];
     uint32_t gathered = CAP + 1;
     if (bin < BINS - 1) {
-      Shared* zero = peer(0);
       const float behind = (float)(bin + 1);
-      each([&](float x, uint32_t i) {
-        if (fast_bin(x) < behind) {
-          const uint32_t at = atomicAdd(&zero->n_cand, 1u);
-          if (at < CAP) zero->cand[at] = place(x, begin + i);
-        }
-      });
+      gather([&](float x, uint32_t) { return fast_bin(x) < behind; });
       cl.sync();
-      gathered = zero->n_cand;
+      gathered = peer(0)->n_cand;
     }
     if (gathered <= CAP) {
       cl.sync();  // the others have read it
@@ -433,7 +535,7 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
         count_range();
       } else {
         // The guess: counts times the weight at a bin's middle, within a margin.
-        double m[4], sum = 0, all;
+        double m[4], sum = 0, all, var = 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const uint64_t b = 4 * tid + j;
@@ -442,9 +544,15 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
                                 : -((float)b + 0.5f) * (float)(RANGE / BINS * 1.4426950408889634);
           m[j] = c[j] ? (double)c[j] * (double)exp2f(y) : 0.0;
           sum += m[j];
+          var += m[j] * m[j];
         }
-        double run = block_before(sum, sh.warp64b, &all);
-        const double want = round ? (goal - (double)above) / UNIT : (double)p.top_p * all, slack = 1e-3 * all;
+        double run = block_before(sum, sh.warp64b, &all), var_all;
+        block_before(var, sh.warp64, &var_all);
+        // A bin's values are off its middle by RANGE / BINS / sqrt(12), all alike where they are few distinct
+        // ones (16-bit logits). Errors of hundreds of bins cancel, and those before and behind the border partly
+        // do: 0.4 of the standard deviation leaves a few bins, and held in every one of 480 simulated rows.
+        const double want = round ? (goal - (double)above) / UNIT : (double)p.top_p * all;
+        const double slack = 0.4 * RANGE / BINS / 3.46 * sqrt(var_all) + 3e-5 * all;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           if (run < want - slack && run + m[j] >= want - slack) sh.found[0] = 4 * tid + j;
@@ -458,24 +566,42 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
         for (int turn = 0;; turn++) {
           uint64_t ma = 0, mi = 0, ml = 0;
           if (everything && !turn) {
+            // Consecutive values, as in the draw, and the range's places collected on the way: the draw then
+            // needs no pass of its own.
             const float fa = (float)try_a, fb = try_b == BINS - 1 ? INFINITY : (float)(try_b + 1);
-            each([&](float x, uint32_t) {
-              const float b = fast_bin(x);
-              const uint64_t w = wt.of(x);
-              ma += b < fa ? w : 0;
-              mi += b >= fa && b < fb ? w : 0;
-              ml += b >= fb ? w : 0;
-            });
+            if (tid == 0) sh.n_here = 0;
+            __syncthreads();
+            for (uint32_t i = i0; i < i1; i += 4) {
+              float x[4];
+              uint64_t w[4];
+#pragma unroll
+              for (int j = 0; j < 4; j++) x[j] = i + j < i1 ? value(vals[i + j]) : -INFINITY;
+#pragma unroll
+              for (int j = 0; j < 4; j++) w[j] = wt.of(x[j]);
+#pragma unroll
+              for (int j = 0; j < 4; j++) {
+                const float b = fast_bin(x[j]);
+                ml += w[j];
+                ma += b < fa ? w[j] : 0;
+                if (b >= fa && b < fb) {
+                  mi += w[j];
+                  const uint32_t at = atomicAdd(&sh.n_here, 1u);
+                  if (at < CAP) local[at] = place(x[j], begin + i + j);
+                }
+              }
+            }
+            ml -= ma + mi;
+            mine = ma;
           } else {
             each([&](float x, uint32_t i) {
               const uint64_t pl = place(x, begin + i);
               if (!(x > -INFINITY) || pl < lo || pl > hi) return;
               const uint32_t b = bin_of(x, pl);
-              if ((round || turn) && b > try_b) return;
+              if (turn ? b < try_a || b > try_b : round && b > try_b) return;
               const uint64_t w = wt.of(x);
-              ma += b < try_a ? w : 0;
-              mi += b >= try_a && b <= try_b ? w : 0;
-              ml += b > try_b ? w : 0;
+              if (b < try_a) ma += w;
+              else if (b <= try_b) mi += w;
+              else ml += w;
             });
           }
           ma = block_sum(ma, sh.warp64);
@@ -484,9 +610,9 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
           slot ^= 5;  // 1 and 4 in turn
           if (tid == 0) sh.post[slot] = ma, sh.post[slot + 1] = mi, sh.post[slot + 2] = ml;
           cl.sync();
-          ma = mi = ml = 0;
-#pragma unroll 8
-          for (uint32_t i = 0; i < CL; i++) ma += peer(i)->post[slot], mi += peer(i)->post[slot + 1], ml += peer(i)->post[slot + 2];
+          uint64_t unused;
+          ma = add_up(slot, unused), mi = add_up(slot + 1, unused), ml = add_up(slot + 2, unused);
+          if (turn) ma = mass_above;  // try_a is bin_a
           if (!round && !turn) goal = (double)p.top_p * (double)(ma + mi + ml);
           const bool begins = try_a == bin_a || above + ma == 0 || (double)(above + ma) < goal;
           const bool ends = try_b == bin_b || (double)(above + ma + mi) >= goal;
@@ -494,6 +620,7 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
           else if (!begins) bin_b = try_a - 1;
           else bin_a = try_b + 1, mass_above = ma + mi;
           count_range();
+          direct = everything && !turn && bin_a == try_a && bin_b == try_b && n_in <= CAP;
           if (n_in <= CAP || bin_a == bin_b) break;
           try_a = bin_a, try_b = (bin_a + bin_b) / 2;
         }
@@ -504,46 +631,29 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
         n_in += n_above, n_above = 0;
       }
       if (n_in <= CAP) {
-        Shared* zero = peer(0);
         const float fa = (float)bin_a, fb = bin_b == BINS - 1 ? INFINITY : (float)(bin_b + 1);
-        each([&](float x, uint32_t i) {
-          if (everything && !(fast_bin(x) >= fa && fast_bin(x) < fb)) return;
-          const uint64_t pl = place(x, begin + i);
-          if (!(x > -INFINITY) || pl < lo || pl > hi) return;
-          const uint32_t b = bin_of(x, pl);
-          if (b >= bin_a && b <= bin_b) zero->cand[atomicAdd(&zero->n_cand, 1u)] = pl;
-        });
+        if (direct) {
+          push(local);
+        } else if (everything) {
+          gather([&](float x, uint32_t) { return x > -INFINITY && fast_bin(x) >= fa && fast_bin(x) < fb; });
+        } else {
+          gather([&](float x, uint32_t i) {
+            const uint64_t pl = place(x, begin + i);
+            if (!(x > -INFINITY) || pl < lo || pl > hi) return false;
+            const uint32_t b = bin_of(x, pl);
+            return b >= bin_a && b <= bin_b;
+          });
+        }
         cl.sync();
         if (small && rank != 0) return;
         if (rank == 0) {
-          order((uint32_t)n_in);
-          uint32_t kept = (uint32_t)n_in;
-          if (!mass) kept = (uint32_t)((uint64_t)p.top_k - above - n_above);
-          constexpr uint32_t PER = CAP / THREADS;
-          uint64_t w[PER], mine = 0, nothing;
-          if (mass) {
-#pragma unroll
-            for (uint32_t j = 0; j < PER; j++) {
-              const uint32_t at = tid * PER + j;
-              w[j] = at < kept ? wt.of(unordered((uint32_t)(sh.sorted[at] >> 32))) : 0;
-              mine += w[j];
-            }
-          }
           if (small) {
-            draw_sorted(kept);
+            order((uint32_t)n_in);
+            draw_sorted((uint32_t)p.top_k);
             return;
           }
-          if (mass) {
-            uint64_t run = above + mass_above + block_before(mine, sh.warp64, &nothing), in = 0;
-#pragma unroll
-            for (uint32_t j = 0; j < PER; j++) {
-              const uint32_t at = tid * PER + j;
-              in += at < kept && ((double)run < goal || n_above + at == 0);
-              run += w[j];
-            }
-            kept = (uint32_t)block_sum(in, sh.warp64b);  // at least one: the range begins before the goal
-          }
-          if (tid == 0) sh.cut = sh.sorted[kept - 1], sh.n_cand = 0;
+          const uint64_t border = border_among((uint32_t)n_in, mass, above + (mass ? mass_above : n_above), mass ? goal : (double)p.top_k);
+          if (tid == 0) sh.cut = border, sh.n_cand = 0;
         }
         cl.sync();
         cut = peer(0)->cut;
@@ -569,29 +679,40 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
     }
   }
 
-  // ---- the draw, in the vocabulary's order: a thread has consecutive values, an odd number (no bank conflicts) ----
-  const uint32_t run_len = (n + THREADS - 1) / THREADS | 1, i0 = min(n, tid * run_len), i1 = min(n, i0 + run_len);
+  // ---- the draw, in the vocabulary's order ----
   const float cut_x = cut ? unordered((uint32_t)(cut >> 32)) : -INFINITY;
   const uint32_t cut_i = ~(uint32_t)cut - begin, best_i = ~(uint32_t)best - begin;  // modulo 2^32, as begin + i is
   auto weight_at = [&](uint32_t i) -> uint64_t {  // 0: not kept
-    const float x = vals[i];
+    const float x = value(vals[i]);
     const uint64_t w = wt.of(x);
     const bool in = x > cut_x || (x == cut_x && begin + i <= cut_i + begin);
     return in && (w >= min_weight || i == best_i) ? w : 0;
   };
-  uint64_t mine = 0;
+  if (direct && min_weight == 0) {
+    // the search's sums: the values before its range, and of the range those kept
+    uint64_t* extra = sh.weight;
+    extra[tid] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < sh.n_here; i += THREADS) {
+      const uint64_t pl = local[i];
+      if (pl >= cut)
+        atomicAdd(reinterpret_cast<unsigned long long*>(&extra[(~(uint32_t)pl - begin) / run_len]),
+                  (unsigned long long)wt.of(unordered((uint32_t)(pl >> 32))));
+    }
+    __syncthreads();
+    mine += extra[tid];
+  } else {
+    mine = 0;
 #pragma unroll 4
-  for (uint32_t i = i0; i < i1; i++) mine += weight_at(i);
+    for (uint32_t i = i0; i < i1; i++) mine += weight_at(i);
+  }
   uint64_t cta;
   uint64_t run = block_before(mine, sh.warp64, &cta);
   if (tid == 0) sh.post[9] = cta;
   cl.sync();
-  uint64_t total = 0;
-  for (uint32_t i = 0; i < CL; i++) {
-    const uint64_t m = peer(i)->post[9];
-    run += i < rank ? m : 0;
-    total += m;
-  }
+  uint64_t before_me;
+  const uint64_t total = add_up(9, before_me);
+  run += before_me;
   cl.sync();  // the others read post
   const double aim = (double)u * (double)total;
   // one thread of the cluster holds the value at which the sum passes the aim; its warp looks for it
@@ -609,22 +730,24 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
         if (lane >= o) upto += y;
       }
       upto += run;
-      if (w && (double)upto > aim && (double)(upto - w) <= aim) finish(begin + i + lane, vals[i + lane], total);
+      if (w && (double)upto > aim && (double)(upto - w) <= aim) finish(begin + i + lane, value(vals[i + lane]), total);
       run = __shfl_sync(~0u, upto, 31);
     }
   }
 }
 
 template <typename T>
-cudaError_t draw_typed(const DrawArgs& a, cudaStream_t st) {
-  uint32_t cl = 8;
-  while ((a.vocab + cl - 1) / cl > 40 * 1024 && cl < MAX_CLUSTER) cl *= 2;
-  while (cl > 1 && a.vocab / cl < 2048) cl /= 2;
+cudaError_t draw_typed(const DrawArgs& a, uint32_t sms, cudaStream_t st) {
+  // CTAs a row: as many as let all rows run at once (two CTAs an SM); at least
+  // what the row needs of shared memory, at most what leaves a CTA 2048 values.
+  uint32_t cl = 1;
+  while (cl < MAX_CLUSTER && ((uint64_t)a.vocab * sizeof(T) > (uint64_t)cl * MAX_PART || ((uint64_t)a.n_rows * cl * (cl < 8 ? 1 : 4) <= sms && a.vocab / (cl * 2) >= 2048)))
+    cl *= 2;
   const uint32_t chunk = ((a.vocab + cl - 1) / cl + 7) / 8 * 8;
-  const size_t smem = sizeof(Shared) + (size_t)chunk * 4;
+  const size_t smem = sizeof(Shared) + (size_t)chunk * sizeof(T);
   auto* kern = draw_kernel<T>;
   static SmemOnce once;
-  cudaError_t e = once.allow((const void*)kern, (int)(sizeof(Shared) + 40 * 1024 * 4 + 64));
+  cudaError_t e = once.allow((const void*)kern, (int)(sizeof(Shared) + 2 * MAX_PART + 64));
   if (e == cudaSuccess && cl > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
@@ -642,12 +765,12 @@ cudaError_t draw_typed(const DrawArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_draw(const DrawArgs& a, cudaStream_t st) {
+cudaError_t launch_draw(const DrawArgs& a, uint32_t sms, cudaStream_t st) {
   if (!a.n_rows) return cudaSuccess;
   switch (a.type) {
-    case ACT_F32: return draw_typed<float>(a, st);
-    case ACT_F16: return draw_typed<__half>(a, st);
-    default: return draw_typed<__nv_bfloat16>(a, st);
+    case ACT_F32: return draw_typed<float>(a, sms, st);
+    case ACT_F16: return draw_typed<__half>(a, sms, st);
+    default: return draw_typed<__nv_bfloat16>(a, sms, st);
   }
 }
 

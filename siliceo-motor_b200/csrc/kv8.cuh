@@ -100,6 +100,6 @@ inline cudaError_t launch_kv8_attn(const Kv8AttnArgs& a, uint32_t type, uint32_t
 }
 // Largest vocabulary launch_draw takes.
 constexpr uint32_t DRAW_MAX_VOCAB = 1u << 19;
-cudaError_t launch_draw(const DrawArgs& a, cudaStream_t st);
+cudaError_t launch_draw(const DrawArgs& a, uint32_t sms, cudaStream_t st);
 
 }  // namespace sm

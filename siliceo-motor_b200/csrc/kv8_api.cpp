@@ -256,7 +256,9 @@ int sm_draw(const void* logits_dev, uint32_t type, uint64_t n_rows, uint64_t ld,
     static_assert(sizeof(sm_draw_params) == sizeof(DrawParams) && sizeof(DrawParams) == 16, "16 bytes a row");
     DrawArgs a{logits_dev, mask_dev, (const DrawParams*)params_dev, u_dev, tokens_dev, logprobs_dev, ld ? ld : vocab,
                (uint32_t)n_rows, (uint32_t)vocab, type};
-    const cudaError_t e = launch_draw(a, (cudaStream_t)stream);
+    int sms = 0;
+    cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, ck.dev);
+    if (e == cudaSuccess) e = launch_draw(a, (uint32_t)sms, (cudaStream_t)stream);
     return e == cudaSuccess ? SM_OK : cuda_error("sm_draw", e);
   });
 }
