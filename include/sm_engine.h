@@ -399,6 +399,11 @@ int sm_kv8_append(const sm_kv8* c, const void* k_dev, const void* v_dev, uint32_
 typedef struct sm_kv8_ws sm_kv8_ws;
 int sm_kv8_ws_new(sm_kv8_ws** out);
 int sm_kv8_ws_free(sm_kv8_ws* w);
+/* Whether a bounded wait inside an sm_kv8_attend with this workspace gave up
+ * (tensor-core work that did not complete) since the last call: waits for
+ * `stream`, then returns SM_ERR_CUDA (those outputs are invalid) and clears
+ * the flag, or SM_OK. */
+int sm_kv8_ws_status(const sm_kv8_ws* w, void* stream);
 
 /* Attention of n_rows query rows ([n_heads][head_dim], ld_q elements apart,
  * 0: contiguous) over the cache; query head h reads KV head

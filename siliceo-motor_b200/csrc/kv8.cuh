@@ -63,6 +63,7 @@ struct Kv8AttnArgs {
   float scale;
   float* part;    // partial results, kv8_attn_part_floats()
   uint32_t* cnt;  // arrival counters, zero between launches, kv8_attn_counters()
+  uint32_t* err;  // set when a bounded wait gave up
 };
 
 struct DrawParams {
@@ -88,8 +89,9 @@ cudaError_t launch_kv8_append(const Kv8& c, const void* k, const void* v, uint32
 // Streaming attention (kv8_attn.cuh), one translation unit a row type.
 constexpr uint32_t KV8_MAX_HD = 128;
 constexpr uint32_t KV8_PART_FLOATS = 16 * (KV8_MAX_HD + 2);  // a partial result of up to 16 rows: o, then m and l
-inline uint64_t kv8_attn_part_floats(uint32_t sms) { return (uint64_t)sms * 2 * KV8_PART_FLOATS; }
-inline uint32_t kv8_attn_counters(uint32_t sms) { return sms; }
+constexpr uint32_t KV8_CHUNK_PART_FLOATS = 128 * (KV8_MAX_HD + 2);  // the tensor-core form's (kv8_chunk.cuh, two CTAs an SM)
+inline uint64_t kv8_attn_part_floats(uint32_t sms) { return (uint64_t)sms * 2 * 2 * KV8_CHUNK_PART_FLOATS; }
+inline uint32_t kv8_attn_counters(uint32_t sms) { return sms * 2; }
 cudaError_t launch_kv8_attn_f32(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st);
 cudaError_t launch_kv8_attn_f16(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st);
 cudaError_t launch_kv8_attn_bf16(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st);

@@ -17,7 +17,8 @@ struct sm_kv8_ws {
   int device = 0;
   uint32_t sms = 0;
   float* part = nullptr;
-  uint32_t* cnt = nullptr;
+  uint32_t* cnt = nullptr;  // the counters, then the error word
+  uint32_t* err() const { return cnt + kv8_attn_counters(sms); }
 };
 
 namespace {
@@ -165,7 +166,7 @@ int sm_kv8_ws_new(sm_kv8_ws** out) {
     auto* w = new sm_kv8_ws;
     w->device = dev;
     w->sms = (uint32_t)sms;
-    const size_t cnt = kv8_attn_counters(w->sms) * sizeof(uint32_t);
+    const size_t cnt = (kv8_attn_counters(w->sms) + 1) * sizeof(uint32_t);
     e = cudaMalloc(&w->part, kv8_attn_part_floats(w->sms) * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&w->cnt, cnt);
     if (e == cudaSuccess) e = cudaMemset(w->cnt, 0, cnt);
@@ -191,6 +192,20 @@ int sm_kv8_ws_free(sm_kv8_ws* w) {
   if (dev != w->device) cudaSetDevice(dev);
   delete w;
   return SM_OK;
+}
+
+int sm_kv8_ws_status(const sm_kv8_ws* w, void* stream) {
+  return guarded("sm_kv8_ws_status", [&]() -> int {
+    if (!w) return arg_error("sm_kv8_ws_status", "null workspace");
+    uint32_t h = 0;
+    cudaError_t e = cudaMemcpyAsync(&h, w->err(), sizeof(h), cudaMemcpyDeviceToHost, (cudaStream_t)stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize((cudaStream_t)stream);
+    if (e == cudaSuccess && h) e = cudaMemsetAsync(w->cnt, 0, (kv8_attn_counters(w->sms) + 1) * sizeof(uint32_t), (cudaStream_t)stream);
+    if (e != cudaSuccess) return cuda_error("sm_kv8_ws_status", e);
+    if (!h) return SM_OK;
+    set_error("sm_kv8_attend: a bounded wait gave up");
+    return SM_ERR_CUDA;
+  });
 }
 
 int sm_kv8_attend(const sm_kv8* c, sm_kv8_ws* ws, const void* q_dev, void* out_dev, uint32_t type, uint64_t n_rows,
@@ -230,7 +245,7 @@ int sm_kv8_attend(const sm_kv8* c, sm_kv8_ws* ws, const void* q_dev, void* out_d
     a.n_seqs = (uint32_t)n_seqs, a.n_rows = (uint32_t)n_rows, a.n_heads = n_heads, a.group = n_heads / c->n_kv_heads;
     a.window = window;
     a.scale = scale;
-    a.part = ws->part, a.cnt = ws->cnt;
+    a.part = ws->part, a.cnt = ws->cnt, a.err = ws->err();
     const cudaError_t e = launch_kv8_attn(a, type, ws->sms, (cudaStream_t)stream);
     return e == cudaSuccess ? SM_OK : cuda_error("sm_kv8_attend", e);
   });

@@ -1,6 +1,9 @@
-// Attention over the 8-bit KV cache for BF16 rows (kv8_attn.cuh).
-#include "kv8_attn.cuh"
+// Attention over the 8-bit KV cache for BF16 rows: few a sequence
+// (kv8_attn.cuh) or many (kv8_chunk.cuh).
+#include "kv8_chunk.cuh"
 
 namespace sm {
-cudaError_t launch_kv8_attn_bf16(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) { return attn_typed<__nv_bfloat16>(a, sms, st); }
+cudaError_t launch_kv8_attn_bf16(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) {
+  return chunk_takes<__nv_bfloat16>(a) ? chunk_typed<__nv_bfloat16>(a, sms, st) : attn_typed<__nv_bfloat16>(a, sms, st);
+}
 }  // namespace sm

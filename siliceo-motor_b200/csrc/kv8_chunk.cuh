@@ -1,0 +1,550 @@
+// Attention over the 8-bit paged KV cache, tensor-core form (many rows a
+// sequence: prompts, chunks of them, long drafts), f16 and bf16 rows.
+// kv8_attn_f16.cu and kv8_attn_bf16.cu instantiate it. The weights, their
+// scaling and the merging of partial results are those of kv8_attn.cuh.
+//
+// A unit is 128 (token, head of the group) rows of one sequence and KV head;
+// a step is 64 positions (two pages). CTA roles:
+//   * eight decode warps read a step's codes (the next step's are in flight
+//     meanwhile), turn them into exact f16 and store them as the B operands:
+//     K rows as they are (K-major), V rows as they are too (N-major: the
+//     transposed operand is the tensor core's work);
+//   * one thread issues S = Q K^T (M 128, N 64, Q in tensor memory) and
+//     O += P V (M 128, N hd, P in tensor memory, over S), one after the other;
+//   * four softmax warps, a row a thread: S from tensor memory, weights, P
+//     back; they rescale O when the running maximum has risen by more than 4x
+//     (weights keep that much room in f16), and write the results.
+// One CTA's scores, weights and products follow one another; the two CTAs of
+// an SM overlap each other's. Per step and CTA the tensor pipe needs 512
+// cycles, the exponentials (16 a cycle) 512, shared memory about 640.
+//
+// Work is the list of all steps of all units; every CTA takes an equal share.
+// A sequence's row blocks alternate between its first and last ones, so that
+// under the causal mask neighbours in the list share the work.
+//
+// Every wait on an mbarrier is bounded; one that gives up sets the workspace's
+// error word and an abort flag, after which the other waits return at once,
+// the CTA waits (bounded) for the MMAs it issued, frees its tensor memory and
+// leaves.
+#pragma once
+#include "kv8_attn.cuh"
+#include "tc_common.cuh"
+#include "umma.cuh"
+
+namespace sm {
+namespace {
+
+constexpr uint32_t CH_ROWS = 128, CH_STEP = 64;
+constexpr uint32_t CH_SOFT = 4, CH_DEC = 8, CH_WARPS = CH_SOFT + CH_DEC + 1, CH_THREADS = CH_WARPS * 32;
+constexpr uint32_t CH_TCOLS = 256, CH_TS = 0, CH_TQ = 64, CH_TO = 128;  // tensor memory: S (and P over it), Q, O
+
+__device__ __forceinline__ void ch_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+__device__ __forceinline__ bool ch_wait(uint64_t* b, uint32_t parity, uint32_t* err, volatile uint32_t* abort) {
+  for (uint32_t n = 0; n < TC_SPIN_MAX; n++) {
+    if (mbar_try(b, parity)) return true;
+    if ((n & 31u) == 31u && *abort) return false;
+  }
+  *abort = 1u;
+  atomicOr(err, 1u);
+  return false;
+}
+
+// A sequence as this kernel walks it: tiles are steps.
+__device__ __forceinline__ Seq chunk_seq_of(const Kv8AttnArgs& a, uint32_t s) {
+  Seq q;
+  const int64_t cap = (int64_t)min(a.table_ld, (uint64_t)(1u << 26)) * KV8_PAGE;
+  q.len = a.lens[s];
+  const int32_t r0 = a.first[s], r1 = a.first[s + 1];
+  q.row0 = min(max(r0, 0), (int32_t)a.n_rows);
+  q.n_rows = max(min(max(r1, 0), (int32_t)a.n_rows) - q.row0, 0);
+  const int64_t held = min(max((int64_t)q.len, (int64_t)0), cap);
+  const int64_t from = a.window ? max((int64_t)0, (int64_t)q.len - q.n_rows + 1 - (int64_t)a.window) : 0;
+  q.lo = (int32_t)(min(from, held) / CH_STEP);
+  q.tiles = max(1, (int32_t)((held + CH_STEP - 1) / CH_STEP) - q.lo);
+  q.units = ((int64_t)q.n_rows * a.group + CH_ROWS - 1) / CH_ROWS * a.c.heads;
+  return q;
+}
+
+// A CTA's part of a unit.
+struct ChunkPiece {
+  int64_t unit, end;            // the unit's first step in the list, and the one behind its last
+  uint32_t seq, head, row0, row_base, rows;
+  int32_t len, pos0;            // the sequence's length, the position of its first row
+  int32_t step, stop;           // steps of it to do (those some row sees)
+  int32_t all_lo, all_hi;       // positions that every row sees
+  bool cut_left, cut_right;
+};
+struct ChunkWalk {
+  int64_t x, x_end, seq_base;
+  uint32_t seq;
+  Seq sq;
+  __device__ bool next(const Kv8AttnArgs& a, ChunkPiece& p) {
+    if (x >= x_end) return false;
+    while (x >= seq_base + sq.units * sq.tiles) {
+      seq_base += sq.units * sq.tiles;
+      sq = chunk_seq_of(a, ++seq);
+    }
+    const int64_t in_seq = x - seq_base;
+    const uint32_t unit = (uint32_t)(in_seq >> 31 ? in_seq / sq.tiles : (int64_t)((uint32_t)in_seq / (uint32_t)sq.tiles));
+    p.unit = seq_base + (int64_t)unit * sq.tiles;
+    p.end = p.unit + sq.tiles;
+    const int64_t stop = min(p.end, x_end);
+    const uint32_t total = (uint32_t)sq.n_rows * a.group, blocks = (total + CH_ROWS - 1) / CH_ROWS;
+    p.head = unit / blocks;
+    const uint32_t j = unit - p.head * blocks, block = j & 1 ? blocks - 1 - j / 2 : j / 2;
+    p.seq = seq;
+    p.row0 = (uint32_t)sq.row0;
+    p.row_base = block * CH_ROWS;
+    p.rows = min(CH_ROWS, total - p.row_base);
+    p.len = sq.len;
+    p.pos0 = sq.len - sq.n_rows;
+    const int32_t pos_a = p.pos0 + (int32_t)(p.row_base / a.group), pos_b = p.pos0 + (int32_t)((p.row_base + p.rows - 1) / a.group);
+    const int64_t w64 = a.window ? (int64_t)a.window : (int64_t)1 << 40;
+    p.all_lo = (int32_t)max((int64_t)0, pos_b + 1 - w64), p.all_hi = min(pos_a + 1, sq.len);
+    const int32_t any_lo = (int32_t)max((int64_t)0, pos_a + 1 - w64), any_hi = min(pos_b + 1, sq.len);
+    p.step = max(sq.lo + (int32_t)(x - p.unit), any_lo / (int32_t)CH_STEP);
+    p.stop = min(sq.lo + (int32_t)(stop - p.unit), (int32_t)(((int64_t)max(any_hi, 0) + CH_STEP - 1) / CH_STEP));
+    p.cut_left = x > p.unit, p.cut_right = stop < p.end;
+    x = stop;
+    return true;
+  }
+};
+
+template <uint32_t FMT, typename T, uint32_t HD>
+__global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnArgs a) {
+  constexpr uint32_t GROUP8 = HD / 8 * 128;        // bytes of 8 positions: 16-byte columns of 8 rows each
+  constexpr uint32_t OPERAND = CH_STEP / 8 * GROUP8;  // bytes of a step's K or V
+  constexpr uint32_t ITEMS = CH_STEP * HD / 16 / (CH_DEC * 32);  // 16-code loads of a decode thread, K or V
+  extern __shared__ float4 attn_smem4[];
+  uint8_t* ops = reinterpret_cast<uint8_t*>(attn_smem4);  // K, K, V, V
+  __shared__ int64_t chunk_base[CH_THREADS + 1];
+  __shared__ int64_t warp_sum[CH_WARPS];
+  __shared__ uint64_t full_k[2], full_v[2], empty_k[2], empty_v[2], s_full, p_full, pv_done, q_full;
+  __shared__ float4 scales[4][2];  // of a step's pages: of K, of V, 1 if the page is there
+  __shared__ ChunkPiece open_piece[2];
+  __shared__ uint32_t open_flag[2], last_flag[2], s_tmem, s_abort_word;
+  volatile uint32_t* abort = &s_abort_word;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&full_k[i], CH_DEC * 32), mbar_init(&full_v[i], CH_DEC * 32);
+      mbar_init(&empty_k[i], 1), mbar_init(&empty_v[i], 1);
+      open_flag[i] = 0;
+    }
+    mbar_init(&s_full, 1), mbar_init(&pv_done, 1);
+    mbar_init(&p_full, CH_SOFT * 32), mbar_init(&q_full, CH_SOFT * 32);
+    *abort = 0u;
+    fence_mbar_init();
+  }
+  if (warp == CH_WARPS - 1) {
+    tmem_alloc(&s_tmem, CH_TCOLS);
+    tmem_relinquish();
+  }
+
+  // ---- the list of steps: prefix sums over the sequences ----
+  const uint32_t per_thread = (a.n_seqs + CH_THREADS - 1) / CH_THREADS;
+  {
+    const uint32_t s0 = min(a.n_seqs, threadIdx.x * per_thread), s1 = min(a.n_seqs, s0 + per_thread);
+    int64_t sum = 0;
+    for (uint32_t s = s0; s < s1; s++) {
+      const Seq q = chunk_seq_of(a, s);
+      sum += q.units * q.tiles;
+    }
+    int64_t x = sum;
+    for (uint32_t o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(~0u, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    int64_t before = 0;
+    for (uint32_t i = 0; i < warp; i++) before += warp_sum[i];
+    chunk_base[threadIdx.x] = before + x - sum;
+    if (threadIdx.x == CH_THREADS - 1) chunk_base[CH_THREADS] = before + x;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  }
+  const uint32_t tb = s_tmem;
+  const int64_t total = chunk_base[CH_THREADS];
+  const int64_t share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)2);
+  ChunkWalk walk;
+  walk.x = min(total, (int64_t)blockIdx.x * share), walk.x_end = min(total, walk.x + share);
+  if (walk.x < walk.x_end) {
+    uint32_t lo = 0, hi = CH_THREADS;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (chunk_base[mid] <= walk.x) lo = mid; else hi = mid;
+    }
+    walk.seq = lo * per_thread, walk.seq_base = chunk_base[lo];
+    walk.sq = chunk_seq_of(a, walk.seq);
+  }
+  ChunkPiece pc;
+  uint32_t it = 0, n_piece = 0;  // steps and pieces (with steps) so far
+
+  if (warp >= CH_SOFT && warp < CH_SOFT + CH_DEC) {
+    // ------------------------------------------------ decode warps
+    const uint32_t tid = threadIdx.x - CH_SOFT * 32;
+    uint4 kr[ITEMS], vr[ITEMS];
+    float2 sc = make_float2(0.f, 0.f);
+    bool there = false;  // threads 0 and 1: the page whose scales they bring
+    auto row_of = [&](uint32_t k) { const uint32_t i = tid + k * CH_DEC * 32; return (i & 7) + (i >> 3) / (HD / 16) * 8; };
+    auto col_of = [&](uint32_t k) { return ((tid + k * CH_DEC * 32) >> 3) % (HD / 16); };
+    auto page_id = [&](const ChunkPiece& p, int32_t pg) {
+      return pg >= 0 && (uint64_t)pg < a.table_ld && pg * (int32_t)KV8_PAGE < p.len ? (uint32_t)a.table[(uint64_t)p.seq * a.table_ld + pg] : ~0u;
+    };
+    auto load = [&](const ChunkPiece& p, int32_t step) {
+#pragma unroll
+      for (uint32_t k = 0; k < ITEMS; k++) {
+        const uint32_t row = row_of(k), id = page_id(p, step * 2 + (int32_t)(row / KV8_PAGE));
+        kr[k] = vr[k] = make_uint4(0, 0, 0, 0);
+        if (id < a.c.n_pages) {
+          const uint8_t* kp = a.c.codes + ((uint64_t)id * a.c.heads + p.head) * 2 * KV8_PAGE * HD + (row % KV8_PAGE) * HD + col_of(k) * 16;
+          kr[k] = __ldg(reinterpret_cast<const uint4*>(kp));
+          if (step * (int32_t)CH_STEP + (int32_t)row < p.len) vr[k] = __ldg(reinterpret_cast<const uint4*>(kp + KV8_PAGE * HD));  // behind the end: anything
+        }
+      }
+      if (tid < 2) {
+        const uint32_t id = page_id(p, step * 2 + (int32_t)tid);
+        there = id < a.c.n_pages;
+        sc = there ? __ldg(reinterpret_cast<const float2*>(a.c.scales) + (uint64_t)id * a.c.heads + p.head) : make_float2(0.f, 0.f);
+      }
+    };
+    auto store = [&](uint8_t* dst, const uint4 (&r)[ITEMS]) {
+#pragma unroll
+      for (uint32_t k = 0; k < ITEMS; k++) {
+        const uint32_t row = row_of(k);
+        uint8_t* at = dst + row / 8 * GROUP8 + col_of(k) * 256 + row % 8 * 16;
+        uint4 lo, hi;
+        decode4<FMT>(r[k].x, lo.x, lo.y), decode4<FMT>(r[k].y, lo.z, lo.w);
+        decode4<FMT>(r[k].z, hi.x, hi.y), decode4<FMT>(r[k].w, hi.z, hi.w);
+        *reinterpret_cast<uint4*>(at) = lo;
+        *reinterpret_cast<uint4*>(at + 128) = hi;
+      }
+    };
+    while (walk.next(a, pc) && !*abort) {
+      if (pc.step >= pc.stop) continue;
+      load(pc, pc.step);
+      for (int32_t step = pc.step; step < pc.stop && !*abort; step++, it++) {
+        const uint32_t st = it & 1;
+        if (it >= 2) ch_wait(&empty_k[st], (it / 2 + 1) & 1, a.err, abort);
+        store(ops + st * OPERAND, kr);
+        if (tid < 2) scales[it & 3][tid] = make_float4(sc.x, sc.y, there ? 1.f : 0.f, 0.f);
+        fence_proxy_async();
+        ch_arrive(&full_k[st]);
+        if (it >= 2) ch_wait(&empty_v[st], (it / 2 + 1) & 1, a.err, abort);
+        store(ops + (2 + st) * OPERAND, vr);
+        if (step + 1 < pc.stop) load(pc, step + 1);
+        fence_proxy_async();
+        ch_arrive(&full_v[st]);
+      }
+    }
+  } else if (warp == CH_WARPS - 1) {
+    // ------------------------------------------------ MMAs
+    if (lane == 0) {
+      const uint32_t s_desc = umma_idesc_f16(CH_ROWS, CH_STEP), o_desc = umma_idesc_f16(CH_ROWS, HD) | 1u << 16;  // B N-major
+      while (walk.next(a, pc) && !*abort) {
+        if (pc.step >= pc.stop) continue;
+        ch_wait(&q_full, n_piece++ & 1, a.err, abort);
+        for (int32_t step = pc.step; step < pc.stop && !*abort; step++, it++) {
+          const uint32_t st = it & 1;
+          ch_wait(&full_k[st], it / 2 & 1, a.err, abort);
+          if (it) ch_wait(&pv_done, (it + 1) & 1, a.err, abort);  // P of the last step is read
+          if (*abort) break;
+          tc_fence_after();
+          const uint64_t kd = umma_desc_k(smem_u32(ops + st * OPERAND), 128, GROUP8);
+#pragma unroll
+          for (uint32_t k = 0; k < HD / 16; k++) umma_ts(tb + CH_TS, tb + CH_TQ + 8 * k, kd + k * (256 >> 4), s_desc, k != 0);
+          umma_commit(&empty_k[st]);
+          umma_commit(&s_full);
+          ch_wait(&full_v[st], it / 2 & 1, a.err, abort);
+          ch_wait(&p_full, it & 1, a.err, abort);
+          if (*abort) break;
+          tc_fence_after();
+          // N-major B: 8 positions x 8 dims are 128 bytes; groups of dims follow one another, groups of positions are GROUP8 apart
+          const uint64_t vd = umma_desc_k(smem_u32(ops + (2 + st) * OPERAND), GROUP8, 128);
+#pragma unroll
+          for (uint32_t k = 0; k < CH_STEP / 16; k++)
+            umma_ts(tb + CH_TO, tb + CH_TS + 8 * k, vd + k * (2 * GROUP8 >> 4), o_desc, step != pc.step || k != 0);
+          umma_commit(&empty_v[st]);
+          umma_commit(&pv_done);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------ softmax warps: a row a thread
+    const uint32_t row = threadIdx.x, tl = tb + (warp * 32 << 16);
+    const int64_t w64 = a.window ? (int64_t)a.window : (int64_t)1 << 40;
+    bool gone = false;  // the CTA gave up: decided by the warp as one, tensor-memory access is warp-wide
+    while (walk.next(a, pc)) {
+      float m = MINM, l = 0.f;
+      const uint32_t r = pc.row_base + min(row, pc.rows - 1), token = r / a.group, hq = pc.head * a.group + r % a.group;
+      if (pc.step < pc.stop && !gone) {
+        const int32_t last_pos = pc.pos0 + (int32_t)token;
+        float mult;
+        {  // the row of Q, times a power of two that brings its largest to [2^14, 2^15), and the scale's sign
+          const uint4* src = reinterpret_cast<const uint4*>((const T*)a.q + (uint64_t)(pc.row0 + token) * a.ld_q + (uint64_t)hq * HD);
+          uint32_t top = 0;
+#pragma unroll 4
+          for (uint32_t i = 0; i < HD / 8; i++) {
+            const uint4 v = src[i];
+            const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(to_f(e[j])) & 0x7FFFFFFFu);
+          }
+          const int ex = (int)(top >> 23) - 127;
+          const int k = top == 0 || ex == 128 ? 0 : min(14 - ex, 126);
+          const float up = __uint_as_float((uint32_t)(k + 127) << 23 | (__float_as_uint(a.scale) & 0x80000000u));
+          mult = a.scale * 1.4426950408889634f / up;
+#pragma unroll
+          for (uint32_t c = 0; c < HD / 32; c++) {
+            uint32_t q[16];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+              const uint4 v = src[c * 4 + i];
+              const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+              for (int j = 0; j < 4; j++) q[i * 4 + j] = row < pc.rows ? pack_half(to_f(e[2 * j]) * up, to_f(e[2 * j + 1]) * up) : 0u;
+            }
+            tmem_st16(tl + CH_TQ + 16 * c, q);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          ch_arrive(&q_full);
+        }
+        for (int32_t step = pc.step; step < pc.stop && !gone; step++, it++) {
+          const bool ok = ch_wait(&full_k[it & 1], it / 2 & 1, a.err, abort)  // the scales
+                          && ch_wait(&s_full, it & 1, a.err, abort);
+          gone = __any_sync(~0u, !ok);
+          if (gone) break;
+          tc_fence_after();
+          const int32_t p0 = step * (int32_t)CH_STEP;
+          float f[2], e[2], back[2], frac[2];
+          bool masked = p0 < pc.all_lo || p0 + (int32_t)CH_STEP > pc.all_hi;
+          bool here[2];
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const float4 sc = scales[it & 3][h];
+            const int ev = min(max((int)(__float_as_uint(sc.y) >> 23 & 255) - 127, -60), 126);
+            e[h] = (float)ev, back[h] = __uint_as_float((uint32_t)(127 - ev) << 23), frac[h] = sc.y * back[h];
+            f[h] = mult * sc.x;
+            here[h] = sc.z != 0.f;
+            masked |= !here[h];
+          }
+          // columns of this row that it sees: [lo, hi) of each page's 32
+          int32_t lo[2] = {0, 0}, hi[2] = {32, 32};
+          if (masked) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const int64_t first = (int64_t)last_pos - w64 + 1 - (p0 + 32 * h);
+              lo[h] = (int32_t)min(max(first, (int64_t)0), (int64_t)32);
+              hi[h] = here[h] ? min(max(last_pos + 1 - (p0 + 32 * h), 0), 32) : 0;
+            }
+          }
+          float top = MINM;
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            uint32_t s[32];
+            tmem_ld32(tl + CH_TS + 32 * h, s);
+            tmem_wait_ld();
+            float x = -INFINITY;
+            if (masked) {
+#pragma unroll
+              for (int i = 0; i < 32; i++) x = fmaxf(x, i >= lo[h] && i < hi[h] ? __uint_as_float(s[i]) : -INFINITY);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i++) x = fmaxf(x, __uint_as_float(s[i]));
+            }
+            if (x > -INFINITY) top = fmaxf(top, x * f[h] + e[h]);
+          }
+          // Weights up to 2^14 fit f16 (times a scale's fraction): the maximum may lag by a factor 4.
+          if (__any_sync(~0u, top > m + 2.f)) {
+            const float mn = top > m + 2.f ? ceilf(top) : m, alpha = ex2(m - mn);
+            m = mn;
+            l *= alpha;
+            if (step != pc.step) {
+#pragma unroll 1
+              for (uint32_t c = 0; c < HD / 32; c++) {
+                uint32_t o[32];
+                tmem_ld32(tl + CH_TO + 32 * c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st32(tl + CH_TO + 32 * c, o);
+              }
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const float c = e[h] - m + 12.f;
+            float sum = 0.f;
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+              uint32_t s[16], p[8];
+              tmem_ld16(tl + CH_TS + 32 * h + 16 * half, s);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                float y[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                  y[j] = ex2(fmaf(__uint_as_float(s[2 * i + j]), f[h], c));
+                  if (masked && !(16 * half + 2 * i + j >= lo[h] && 16 * half + 2 * i + j < hi[h])) y[j] = 0.f;
+                  sum += y[j];
+                  y[j] *= frac[h];
+                  if (masked && !(16 * half + 2 * i + j >= lo[h] && 16 * half + 2 * i + j < hi[h])) y[j] = 0.f;  // frac may be NaN
+                }
+                p[i] = pack_half(y[0], y[1]);
+              }
+              tmem_st8(tl + CH_TS + 16 * h + 8 * half, p);  // over columns already read
+            }
+            l = fmaf(sum, back[h], l);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          ch_arrive(&p_full);
+        }
+        if (!gone) gone = __any_sync(~0u, !ch_wait(&pv_done, (it + 1) & 1, a.err, abort));
+        tc_fence_after();
+      }
+      // ---- this piece's row ----
+      const bool whole = !pc.cut_left && !pc.cut_right, some = pc.step < pc.stop;
+      const uint32_t side = pc.cut_left ? 0 : 1;
+      float* gpart = a.part + ((uint64_t)blockIdx.x * 2 + side) * KV8_CHUNK_PART_FLOATS;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T* dst = (T*)a.out + (uint64_t)(pc.row0 + token) * a.ld_out + (uint64_t)hq * HD;
+#pragma unroll 1
+      for (uint32_t c = 0; c < HD / 16; c++) {
+        uint32_t o[16];
+        if (some) {
+          tmem_ld16(tl + CH_TO + 16 * c, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; i++) o[i] = 0;
+        }
+        if (row >= pc.rows || gone) {
+        } else if (whole) {
+          T v[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) from_f(__uint_as_float(o[i]) * inv, v[i]);
+          reinterpret_cast<uint4*>(dst + 16 * c)[0] = reinterpret_cast<uint4*>(v)[0];
+          reinterpret_cast<uint4*>(dst + 16 * c)[1] = reinterpret_cast<uint4*>(v)[1];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            __stcg(reinterpret_cast<uint4*>(gpart + row * HD + 16 * c) + i, make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+        }
+        __syncwarp();
+      }
+      if (!whole) {
+        if (row < pc.rows) __stcg(reinterpret_cast<float2*>(gpart + CH_ROWS * KV8_MAX_HD) + row, make_float2(m, l));
+        if (row == 0) open_piece[side] = pc, open_flag[side] = 1;
+      }
+      tc_fence_before();  // O and Q are read before the next piece's MMAs
+    }
+  }
+
+  // ---- teardown: the MMAs are complete (softmax waited for the last), or the CTA gave up and waits for them ----
+  __syncwarp();
+  if (*abort && warp == CH_WARPS - 1 && lane == 0) {
+    umma_commit(&s_full);  // its phase changes once more when all MMAs issued are complete
+    for (uint32_t n = 0; n < 1000; n++) mbar_try(&s_full, it & 1);
+  }
+  __syncwarp();
+  __threadfence();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == CH_WARPS - 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tb, CH_TCOLS);
+  }
+
+  // ---- units cut between CTAs: the last one to arrive merges, in CTA order ----
+  if (!open_flag[0] && !open_flag[1]) return;
+  if (threadIdx.x < 2) {
+    uint32_t last = 0;
+    if (open_flag[threadIdx.x]) {
+      const ChunkPiece& p = open_piece[threadIdx.x];
+      const int64_t c0 = p.unit / share;
+      const uint32_t others = (uint32_t)((p.end - 1) / share - c0);
+      last = atomicInc(a.cnt + c0, others) == others;
+    }
+    last_flag[threadIdx.x] = last;
+  }
+  __syncthreads();
+  for (int side = 0; side < 2; side++) {
+    if (!last_flag[side]) continue;
+    __threadfence();
+    const ChunkPiece& p = open_piece[side];
+    const int64_t c0 = p.unit / share;
+    const uint32_t others = (uint32_t)((p.end - 1) / share - c0);
+    for (uint32_t at = threadIdx.x; at < p.rows * (HD / 4); at += CH_THREADS) {
+      const uint32_t row = at / (HD / 4), d = at % (HD / 4) * 4;
+      float m = MINM, l = 0.f;
+      float4 o = make_float4(0, 0, 0, 0);
+      for (uint32_t c = 0; c <= others; c += 4) {
+        float2 ml[4];
+        float4 v[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+          ml[k] = make_float2(MINM, 0.f);
+          v[k] = make_float4(0, 0, 0, 0);
+          if (c + k <= others) {
+            const float* part = a.part + ((uint64_t)(c0 + c + k) * 2 + (c + k ? 0 : 1)) * KV8_CHUNK_PART_FLOATS;
+            ml[k] = __ldcg(reinterpret_cast<const float2*>(part + CH_ROWS * KV8_MAX_HD) + row);
+            v[k] = __ldcg(reinterpret_cast<const float4*>(part + row * HD + d));
+          }
+        }
+        float mn = m;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) mn = fmaxf(mn, ml[k].x);
+        const float f0 = ex2(m - mn);
+        l *= f0, o.x *= f0, o.y *= f0, o.z *= f0, o.w *= f0;
+        m = mn;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+          const float f = ex2(ml[k].x - m);
+          l += f * ml[k].y;
+          o.x += f * v[k].x, o.y += f * v[k].y, o.z += f * v[k].z, o.w += f * v[k].w;
+        }
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const uint32_t r = p.row_base + row;
+      T v[4];
+      from_f(o.x * inv, v[0]), from_f(o.y * inv, v[1]), from_f(o.z * inv, v[2]), from_f(o.w * inv, v[3]);
+      *reinterpret_cast<uint2*>((T*)a.out + (uint64_t)(p.row0 + r / a.group) * a.ld_out + (uint64_t)(p.head * a.group + r % a.group) * HD + d) =
+          *reinterpret_cast<uint2*>(v);
+    }
+  }
+}
+
+template <uint32_t FMT, typename T, uint32_t HD>
+cudaError_t chunk_launch(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) {
+  constexpr uint32_t smem = 4 * CH_STEP * HD * 2;
+  auto* kern = kv8_chunk_kernel<FMT, T, HD>;
+  static SmemOnce once;
+  const cudaError_t e = once.allow((const void*)kern, (int)smem);
+  if (e != cudaSuccess) return e;
+  kern<<<2 * sms, CH_THREADS, smem, st>>>(a);
+  return cudaGetLastError();
+}
+
+// Rows of a sequence, on average, from which this form is taken.
+constexpr uint32_t CHUNK_MIN_ROWS = 33;
+template <typename T>
+bool chunk_takes(const Kv8AttnArgs& a) {
+  return (a.c.hd == 64 || a.c.hd == 128) && (uint64_t)a.n_rows * a.group >= (uint64_t)CHUNK_MIN_ROWS * a.n_seqs;
+}
+template <typename T>
+cudaError_t chunk_typed(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) {
+  if (a.c.hd == 64) return a.c.fmt == KV8_E4M3 ? chunk_launch<KV8_E4M3, T, 64>(a, sms, st) : chunk_launch<KV8_I8, T, 64>(a, sms, st);
+  return a.c.fmt == KV8_E4M3 ? chunk_launch<KV8_E4M3, T, 128>(a, sms, st) : chunk_launch<KV8_I8, T, 128>(a, sms, st);
+}
+
+}  // namespace
+}  // namespace sm

@@ -167,6 +167,7 @@ SIGNATURES = {
     "sm_kv8_append": (C.c_int, [C.POINTER(sm_kv8), P, P, U32, U64, U64, U64, P, P]),
     "sm_kv8_ws_new": (C.c_int, [C.POINTER(P)]),
     "sm_kv8_ws_free": (C.c_int, [P]),
+    "sm_kv8_ws_status": (C.c_int, [P, P]),
     "sm_kv8_attend": (C.c_int, [C.POINTER(sm_kv8), P, P, P, U32, U64, U32, U64, U64, U64, P, P, P, U64, C.c_float, U32, P]),
     "sm_draw": (C.c_int, [P, U32, U64, U64, U64, P, P, P, P, P, P]),
     "sm_synth_preset": (C.c_int, [C.c_int, C.POINTER(sm_synth_spec)]),
@@ -672,6 +673,10 @@ class Kv8Workspace:
         out = C.c_void_p()
         _check(lib().sm_kv8_ws_new(C.byref(out)))
         self.h = out
+
+    def status(self, stream: int = 0) -> None:
+        """Raises if a bounded wait in an earlier attend() with this workspace gave up."""
+        _check(lib().sm_kv8_ws_status(self.h, stream))
 
     def free(self) -> None:
         if self.h:
