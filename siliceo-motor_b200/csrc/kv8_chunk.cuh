@@ -31,6 +31,8 @@
 #include "tc_common.cuh"
 #include "umma.cuh"
 
+#include <type_traits>
+
 namespace sm {
 namespace {
 
@@ -43,7 +45,10 @@ __device__ __forceinline__ void ch_arrive(uint64_t* b) {
 }
 __device__ __forceinline__ bool ch_wait(uint64_t* b, uint32_t parity, uint32_t* err, volatile uint32_t* abort) {
   for (uint32_t n = 0; n < TC_SPIN_MAX; n++) {
-    if (mbar_try(b, parity)) return true;
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok) : "r"(smem_u32(b)), "r"(parity) : "memory");
+    if (ok) return true;
     if ((n & 31u) == 31u && *abort) return false;
   }
   *abort = 1u;
@@ -116,7 +121,7 @@ template <uint32_t FMT, typename T, uint32_t HD>
 __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnArgs a) {
   constexpr uint32_t GROUP8 = HD / 8 * 128;        // bytes of 8 positions: 16-byte columns of 8 rows each
   constexpr uint32_t OPERAND = CH_STEP / 8 * GROUP8;  // bytes of a step's K or V
-  constexpr uint32_t ITEMS = CH_STEP * HD / 16 / (CH_DEC * 32);  // 16-code loads of a decode thread, K or V
+  constexpr uint32_t ITEMS = CH_STEP * HD / 16 / 128;  // 16-code loads of a decode thread
   extern __shared__ float4 attn_smem4[];
   uint8_t* ops = reinterpret_cast<uint8_t*>(attn_smem4);  // K, K, V, V
   __shared__ int64_t chunk_base[CH_THREADS + 1];
@@ -130,7 +135,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; i++) {
-      mbar_init(&full_k[i], CH_DEC * 32), mbar_init(&full_v[i], CH_DEC * 32);
+      mbar_init(&full_k[i], CH_DEC * 16), mbar_init(&full_v[i], CH_DEC * 16);
       mbar_init(&empty_k[i], 1), mbar_init(&empty_v[i], 1);
       open_flag[i] = 0;
     }
@@ -186,60 +191,69 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
   uint32_t it = 0, n_piece = 0;  // steps and pieces (with steps) so far
 
   if (warp >= CH_SOFT && warp < CH_SOFT + CH_DEC) {
-    // ------------------------------------------------ decode warps
-    const uint32_t tid = threadIdx.x - CH_SOFT * 32;
-    uint4 kr[ITEMS], vr[ITEMS];
-    float2 sc = make_float2(0.f, 0.f);
-    bool there = false;  // threads 0 and 1: the page whose scales they bring
-    auto row_of = [&](uint32_t k) { const uint32_t i = tid + k * CH_DEC * 32; return (i & 7) + (i >> 3) / (HD / 16) * 8; };
-    auto col_of = [&](uint32_t k) { return ((tid + k * CH_DEC * 32) >> 3) % (HD / 16); };
-    auto page_id = [&](const ChunkPiece& p, int32_t pg) {
-      return pg >= 0 && (uint64_t)pg < a.table_ld && pg * (int32_t)KV8_PAGE < p.len ? (uint32_t)a.table[(uint64_t)p.seq * a.table_ld + pg] : ~0u;
+    // ------------------------------------------------ decode warps: four for K, four for V
+    const uint32_t tid = threadIdx.x % 128, is_v = warp >= CH_SOFT + CH_DEC / 2;
+    uint64_t *full = is_v ? full_v : full_k, *empty = is_v ? empty_v : empty_k;
+    uint8_t* dst = ops + is_v * 2 * OPERAND;
+    // An item is 16 codes of a row; a thread's are 128 apart, 8 rows side by side in a warp.
+    const uint32_t row0 = (tid & 7) + (tid >> 3) / (HD / 16) * 8, col = (tid >> 3) % (HD / 16);
+    constexpr uint32_t ROWS = 128 / (HD / 16);  // rows between items
+    const uint64_t src0 = ((uint64_t)is_v * KV8_PAGE + row0) * HD + col * 16;
+    struct Ids { uint32_t id[2]; };  // a step's pages
+    auto pages = [&](const ChunkPiece& p, int32_t step) {
+      Ids r;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int32_t pg = step * 2 + h;
+        r.id[h] = step < p.stop && (uint64_t)pg < a.table_ld && pg * (int32_t)KV8_PAGE < p.len ? (uint32_t)a.table[(uint64_t)p.seq * a.table_ld + pg] : ~0u;
+      }
+      return r;
     };
-    auto load = [&](const ChunkPiece& p, int32_t step) {
+    auto load = [&](const ChunkPiece& p, int32_t step, const Ids& ids, uint4 (&r)[ITEMS]) {
 #pragma unroll
       for (uint32_t k = 0; k < ITEMS; k++) {
-        const uint32_t row = row_of(k), id = page_id(p, step * 2 + (int32_t)(row / KV8_PAGE));
-        kr[k] = vr[k] = make_uint4(0, 0, 0, 0);
-        if (id < a.c.n_pages) {
-          const uint8_t* kp = a.c.codes + ((uint64_t)id * a.c.heads + p.head) * 2 * KV8_PAGE * HD + (row % KV8_PAGE) * HD + col_of(k) * 16;
-          kr[k] = __ldg(reinterpret_cast<const uint4*>(kp));
-          if (step * (int32_t)CH_STEP + (int32_t)row < p.len) vr[k] = __ldg(reinterpret_cast<const uint4*>(kp + KV8_PAGE * HD));  // behind the end: anything
-        }
-      }
-      if (tid < 2) {
-        const uint32_t id = page_id(p, step * 2 + (int32_t)tid);
-        there = id < a.c.n_pages;
-        sc = there ? __ldg(reinterpret_cast<const float2*>(a.c.scales) + (uint64_t)id * a.c.heads + p.head) : make_float2(0.f, 0.f);
+        const uint32_t row = row0 + k * ROWS, id = ids.id[k * ROWS / KV8_PAGE];
+        r[k] = make_uint4(0, 0, 0, 0);
+        // V behind the sequence's end: anything lies there
+        if (id < a.c.n_pages && (!is_v || step * (int32_t)CH_STEP + (int32_t)row < p.len))
+          r[k] = __ldg(reinterpret_cast<const uint4*>(a.c.codes + ((uint64_t)id * a.c.heads + p.head) * 2 * KV8_PAGE * HD + src0 + (k * ROWS) % KV8_PAGE * HD));
       }
     };
-    auto store = [&](uint8_t* dst, const uint4 (&r)[ITEMS]) {
+    auto put = [&](const ChunkPiece& p, const Ids& ids, const uint4 (&r)[ITEMS]) {
+      const uint32_t st = it & 1;
+      float2 sc = make_float2(0.f, 0.f);
+      const bool brings = !is_v && tid < 2, there = brings && ids.id[tid & 1] < a.c.n_pages;
+      if (there) sc = __ldg(reinterpret_cast<const float2*>(a.c.scales) + (uint64_t)ids.id[tid & 1] * a.c.heads + p.head);
+      if (it >= 2) ch_wait(&empty[st], (it / 2 + 1) & 1, a.err, abort);
 #pragma unroll
       for (uint32_t k = 0; k < ITEMS; k++) {
-        const uint32_t row = row_of(k);
-        uint8_t* at = dst + row / 8 * GROUP8 + col_of(k) * 256 + row % 8 * 16;
+        uint8_t* at = dst + st * OPERAND + (row0 + k * ROWS) / 8 * GROUP8 + col * 256 + row0 % 8 * 16;
         uint4 lo, hi;
         decode4<FMT>(r[k].x, lo.x, lo.y), decode4<FMT>(r[k].y, lo.z, lo.w);
         decode4<FMT>(r[k].z, hi.x, hi.y), decode4<FMT>(r[k].w, hi.z, hi.w);
         *reinterpret_cast<uint4*>(at) = lo;
         *reinterpret_cast<uint4*>(at + 128) = hi;
       }
+      if (brings) scales[it & 3][tid] = make_float4(sc.x, sc.y, there ? 1.f : 0.f, 0.f);
+      fence_proxy_async();
+      ch_arrive(&full[st]);
+      it++;
     };
     while (walk.next(a, pc) && !*abort) {
       if (pc.step >= pc.stop) continue;
-      load(pc, pc.step);
-      for (int32_t step = pc.step; step < pc.stop && !*abort; step++, it++) {
-        const uint32_t st = it & 1;
-        if (it >= 2) ch_wait(&empty_k[st], (it / 2 + 1) & 1, a.err, abort);
-        store(ops + st * OPERAND, kr);
-        if (tid < 2) scales[it & 3][tid] = make_float4(sc.x, sc.y, there ? 1.f : 0.f, 0.f);
-        fence_proxy_async();
-        ch_arrive(&full_k[st]);
-        if (it >= 2) ch_wait(&empty_v[st], (it / 2 + 1) & 1, a.err, abort);
-        store(ops + (2 + st) * OPERAND, vr);
-        if (step + 1 < pc.stop) load(pc, step + 1);
-        fence_proxy_async();
-        ch_arrive(&full_v[st]);
+      // codes one step ahead, page ids two
+      uint4 r0[ITEMS], r1[ITEMS];
+      Ids i0 = pages(pc, pc.step), i1 = pages(pc, pc.step + 1);
+      load(pc, pc.step, i0, r0);
+      for (int32_t step = pc.step; step < pc.stop && !*abort; step += 2) {
+        load(pc, step + 1, i1, r1);
+        const Ids i2 = pages(pc, step + 2);
+        put(pc, i0, r0);
+        if (step + 1 >= pc.stop) break;
+        load(pc, step + 2, i2, r0);
+        const Ids i3 = pages(pc, step + 3);
+        put(pc, i1, r1);
+        i0 = i2, i1 = i3;
       }
     }
   } else if (warp == CH_WARPS - 1) {
@@ -345,21 +359,20 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
             }
           }
           float top = MINM;
+          auto largest = [&](auto with_mask) {
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            uint32_t s[32];
-            tmem_ld32(tl + CH_TS + 32 * h, s);
-            tmem_wait_ld();
-            float x = -INFINITY;
-            if (masked) {
+            for (int h = 0; h < 2; h++) {
+              uint32_t s[32];
+              tmem_ld32(tl + CH_TS + 32 * h, s);
+              tmem_wait_ld();
+              float x = -INFINITY;
 #pragma unroll
-              for (int i = 0; i < 32; i++) x = fmaxf(x, i >= lo[h] && i < hi[h] ? __uint_as_float(s[i]) : -INFINITY);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; i++) x = fmaxf(x, __uint_as_float(s[i]));
+              for (int i = 0; i < 32; i++)
+                x = fmaxf(x, !with_mask.value || (i >= lo[h] && i < hi[h]) ? __uint_as_float(s[i]) : -INFINITY);
+              if (x > -INFINITY) top = fmaxf(top, x * f[h] + e[h]);
             }
-            if (x > -INFINITY) top = fmaxf(top, x * f[h] + e[h]);
-          }
+          };
+          if (masked) largest(std::true_type{}); else largest(std::false_type{});
           // Weights up to 2^14 fit f16 (times a scale's fraction): the maximum may lag by a factor 4.
           if (__any_sync(~0u, top > m + 2.f)) {
             const float mn = top > m + 2.f ? ceilf(top) : m, alpha = ex2(m - mn);
@@ -377,32 +390,36 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
               }
             }
           }
+          auto weigh = [&](auto with_mask) {
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const float c = e[h] - m + 12.f;
-            float sum = 0.f;
+            for (int h = 0; h < 2; h++) {
+              const float c = e[h] - m + 12.f;
+              float sum = 0.f;
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-              uint32_t s[16], p[8];
-              tmem_ld16(tl + CH_TS + 32 * h + 16 * half, s);
-              tmem_wait_ld();
+              for (int half = 0; half < 2; half++) {
+                uint32_t s[16], p[8];
+                tmem_ld16(tl + CH_TS + 32 * h + 16 * half, s);
+                tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 8; i++) {
-                float y[2];
+                for (int i = 0; i < 8; i++) {
+                  float y[2];
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                  y[j] = ex2(fmaf(__uint_as_float(s[2 * i + j]), f[h], c));
-                  if (masked && !(16 * half + 2 * i + j >= lo[h] && 16 * half + 2 * i + j < hi[h])) y[j] = 0.f;
-                  sum += y[j];
-                  y[j] *= frac[h];
-                  if (masked && !(16 * half + 2 * i + j >= lo[h] && 16 * half + 2 * i + j < hi[h])) y[j] = 0.f;  // frac may be NaN
+                  for (int j = 0; j < 2; j++) {
+                    const int col = 16 * half + 2 * i + j;
+                    const bool see = !with_mask.value || (col >= lo[h] && col < hi[h]);
+                    y[j] = ex2(fmaf(__uint_as_float(s[2 * i + j]), f[h], c));
+                    if (!see) y[j] = 0.f;
+                    sum += y[j];
+                    y[j] = see ? y[j] * frac[h] : 0.f;  // frac may be NaN
+                  }
+                  p[i] = pack_half(y[0], y[1]);
                 }
-                p[i] = pack_half(y[0], y[1]);
+                tmem_st8(tl + CH_TS + 16 * h + 8 * half, p);  // over columns already read
               }
-              tmem_st8(tl + CH_TS + 16 * h + 8 * half, p);  // over columns already read
+              l = fmaf(sum, back[h], l);
             }
-            l = fmaf(sum, back[h], l);
-          }
+          };
+          if (masked) weigh(std::true_type{}); else weigh(std::false_type{});
           tmem_wait_st();
           tc_fence_before();
           ch_arrive(&p_full);
