@@ -43,17 +43,30 @@ constexpr uint32_t CH_TCOLS = 256, CH_TS = 0, CH_TQ = 64, CH_TO = 128;  // tenso
 __device__ __forceinline__ void ch_arrive(uint64_t* b) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
 }
+// One try (the hardware parks the warp for a while), and a bounded wait; a wait
+// that is not urgent sleeps between tries, so that it takes no issue slots.
+__device__ __forceinline__ bool ch_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok) : "r"(smem_u32(b)), "r"(parity) : "memory");
+  return ok;
+}
+template <bool URGENT>
 __device__ __forceinline__ bool ch_wait(uint64_t* b, uint32_t parity, uint32_t* err, volatile uint32_t* abort) {
   for (uint32_t n = 0; n < TC_SPIN_MAX; n++) {
-    uint32_t ok;
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                 : "=r"(ok) : "r"(smem_u32(b)), "r"(parity) : "memory");
-    if (ok) return true;
+    if (ch_try(b, parity)) return true;
+    if (!URGENT) __nanosleep(100);
     if ((n & 31u) == 31u && *abort) return false;
   }
   *abort = 1u;
   atomicOr(err, 1u);
   return false;
+}
+__device__ __forceinline__ void ch_bar(uint32_t id, uint32_t n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ bool ch_elect() {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xFFFFFFFF; selp.u32 %0, 1, 0, p; }" : "=r"(ok));
+  return ok;
 }
 
 // A sequence as this kernel walks it: tiles are steps.
@@ -129,7 +142,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
   __shared__ uint64_t full_k[2], full_v[2], empty_k[2], empty_v[2], s_full, p_full, pv_done, q_full;
   __shared__ float4 scales[4][2];  // of a step's pages: of K, of V, 1 if the page is there
   __shared__ ChunkPiece open_piece[2];
-  __shared__ uint32_t open_flag[2], last_flag[2], s_tmem, s_abort_word;
+  __shared__ uint32_t open_flag[2], last_flag[2], s_tmem, s_abort_word, s_gone;
   volatile uint32_t* abort = &s_abort_word;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
@@ -224,7 +237,9 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
       float2 sc = make_float2(0.f, 0.f);
       const bool brings = !is_v && tid < 2, there = brings && ids.id[tid & 1] < a.c.n_pages;
       if (there) sc = __ldg(reinterpret_cast<const float2*>(a.c.scales) + (uint64_t)ids.id[tid & 1] * a.c.heads + p.head);
-      if (it >= 2) ch_wait(&empty[st], (it / 2 + 1) & 1, a.err, abort);
+      // one warp of the four waits, the others for it at a barrier
+      if (it >= 2 && tid < 32) ch_wait<false>(&empty[st], (it / 2 + 1) & 1, a.err, abort);
+      if (is_v) ch_bar(3, 128); else ch_bar(2, 128);
 #pragma unroll
       for (uint32_t k = 0; k < ITEMS; k++) {
         uint8_t* at = dst + st * OPERAND + (row0 + k * ROWS) / 8 * GROUP8 + col * 256 + row0 % 8 * 16;
@@ -239,13 +254,15 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
       ch_arrive(&full[st]);
       it++;
     };
-    while (walk.next(a, pc) && !*abort) {
+    // No early way out here: the four warps meet at a barrier each step, and after a wait that gave up
+    // (abort is set) the rest of the waits end at once.
+    while (walk.next(a, pc)) {
       if (pc.step >= pc.stop) continue;
       // codes one step ahead, page ids two
       uint4 r0[ITEMS], r1[ITEMS];
       Ids i0 = pages(pc, pc.step), i1 = pages(pc, pc.step + 1);
       load(pc, pc.step, i0, r0);
-      for (int32_t step = pc.step; step < pc.stop && !*abort; step += 2) {
+      for (int32_t step = pc.step; step < pc.stop; step += 2) {
         load(pc, step + 1, i1, r1);
         const Ids i2 = pages(pc, step + 2);
         put(pc, i0, r0);
@@ -257,42 +274,50 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
       }
     }
   } else if (warp == CH_WARPS - 1) {
-    // ------------------------------------------------ MMAs
-    if (lane == 0) {
-      const uint32_t s_desc = umma_idesc_f16(CH_ROWS, CH_STEP), o_desc = umma_idesc_f16(CH_ROWS, HD) | 1u << 16;  // B N-major
-      while (walk.next(a, pc) && !*abort) {
-        if (pc.step >= pc.stop) continue;
-        ch_wait(&q_full, n_piece++ & 1, a.err, abort);
-        for (int32_t step = pc.step; step < pc.stop && !*abort; step++, it++) {
-          const uint32_t st = it & 1;
-          ch_wait(&full_k[st], it / 2 & 1, a.err, abort);
-          if (it) ch_wait(&pv_done, (it + 1) & 1, a.err, abort);  // P of the last step is read
-          if (*abort) break;
-          tc_fence_after();
-          const uint64_t kd = umma_desc_k(smem_u32(ops + st * OPERAND), 128, GROUP8);
+    // ------------------------------------------------ MMAs: the warp as one, an elected lane issues
+    const uint32_t s_desc = umma_idesc_f16(CH_ROWS, CH_STEP), o_desc = umma_idesc_f16(CH_ROWS, HD) | 1u << 16;  // B N-major
+    const uint64_t k_base = umma_desc_k(smem_u32(ops), 128, GROUP8);
+    // N-major B: 8 positions x 8 dims are 128 bytes; groups of dims follow one another, groups of positions are GROUP8 apart
+    const uint64_t v_base = umma_desc_k(smem_u32(ops + 2 * OPERAND), GROUP8, 128);
+    bool gone = false;
+    while (walk.next(a, pc) && !gone) {
+      if (pc.step >= pc.stop) continue;
+      gone = __any_sync(~0u, !ch_wait<true>(&q_full, n_piece++ & 1, a.err, abort));
+      for (int32_t step = pc.step; step < pc.stop && !gone; step++, it++) {
+        const uint32_t st = it & 1;
+        bool ok = ch_wait<true>(&full_k[st], it / 2 & 1, a.err, abort);
+        if (it) ok = ok && ch_wait<true>(&pv_done, (it + 1) & 1, a.err, abort);  // P of the last step is read
+        gone = __any_sync(~0u, !ok);
+        if (gone) break;
+        tc_fence_after();
+        const uint64_t kd = k_base + st * (OPERAND >> 4), vd = v_base + st * (OPERAND >> 4);
+        if (ch_elect()) {
 #pragma unroll
           for (uint32_t k = 0; k < HD / 16; k++) umma_ts(tb + CH_TS, tb + CH_TQ + 8 * k, kd + k * (256 >> 4), s_desc, k != 0);
-          umma_commit(&empty_k[st]);
           umma_commit(&s_full);
-          ch_wait(&full_v[st], it / 2 & 1, a.err, abort);
-          ch_wait(&p_full, it & 1, a.err, abort);
-          if (*abort) break;
-          tc_fence_after();
-          // N-major B: 8 positions x 8 dims are 128 bytes; groups of dims follow one another, groups of positions are GROUP8 apart
-          const uint64_t vd = umma_desc_k(smem_u32(ops + (2 + st) * OPERAND), GROUP8, 128);
+          umma_commit(&empty_k[st]);
+        }
+        __syncwarp();
+        ok = ch_wait<true>(&full_v[st], it / 2 & 1, a.err, abort) && ch_wait<true>(&p_full, it & 1, a.err, abort);
+        gone = __any_sync(~0u, !ok);
+        if (gone) break;
+        tc_fence_after();
+        const uint32_t more = step != pc.step;
+        if (ch_elect()) {
 #pragma unroll
           for (uint32_t k = 0; k < CH_STEP / 16; k++)
-            umma_ts(tb + CH_TO, tb + CH_TS + 8 * k, vd + k * (2 * GROUP8 >> 4), o_desc, step != pc.step || k != 0);
-          umma_commit(&empty_v[st]);
+            umma_ts(tb + CH_TO, tb + CH_TS + 8 * k, vd + k * (2 * GROUP8 >> 4), o_desc, k != 0 ? 1u : more);
           umma_commit(&pv_done);
+          umma_commit(&empty_v[st]);
         }
+        __syncwarp();
       }
     }
   } else {
     // ------------------------------------------------ softmax warps: a row a thread
     const uint32_t row = threadIdx.x, tl = tb + (warp * 32 << 16);
     const int64_t w64 = a.window ? (int64_t)a.window : (int64_t)1 << 40;
-    bool gone = false;  // the CTA gave up: decided by the warp as one, tensor-memory access is warp-wide
+    bool gone = false;  // the CTA gave up: decided by the four warps as one, tensor-memory access is warp-wide
     while (walk.next(a, pc)) {
       float m = MINM, l = 0.f;
       const uint32_t r = pc.row_base + min(row, pc.rows - 1), token = r / a.group, hq = pc.head * a.group + r % a.group;
@@ -330,9 +355,14 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
           ch_arrive(&q_full);
         }
         for (int32_t step = pc.step; step < pc.stop && !gone; step++, it++) {
-          const bool ok = ch_wait(&full_k[it & 1], it / 2 & 1, a.err, abort)  // the scales
-                          && ch_wait(&s_full, it & 1, a.err, abort);
-          gone = __any_sync(~0u, !ok);
+          // one warp waits (full_k: for the scales), the others for it at a barrier
+          if (warp == 0) {
+            ch_wait<true>(&full_k[it & 1], it / 2 & 1, a.err, abort);
+            ch_wait<true>(&s_full, it & 1, a.err, abort);
+            if (lane == 0) s_gone = *abort;
+          }
+          ch_bar(1, CH_SOFT * 32);
+          gone = s_gone;
           if (gone) break;
           tc_fence_after();
           const int32_t p0 = step * (int32_t)CH_STEP;
@@ -424,7 +454,14 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
           tc_fence_before();
           ch_arrive(&p_full);
         }
-        if (!gone) gone = __any_sync(~0u, !ch_wait(&pv_done, (it + 1) & 1, a.err, abort));
+        if (!gone) {
+          if (warp == 0) {
+            ch_wait<true>(&pv_done, (it + 1) & 1, a.err, abort);
+            if (lane == 0) s_gone = *abort;
+          }
+          ch_bar(1, CH_SOFT * 32);
+          gone = s_gone;
+        }
         tc_fence_after();
       }
       // ---- this piece's row ----
@@ -467,7 +504,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
 
   // ---- teardown: the MMAs are complete (softmax waited for the last), or the CTA gave up and waits for them ----
   __syncwarp();
-  if (*abort && warp == CH_WARPS - 1 && lane == 0) {
+  if (*abort && warp == CH_WARPS - 1 && ch_elect()) {
     umma_commit(&s_full);  // its phase changes once more when all MMAs issued are complete
     for (uint32_t n = 0; n < 1000; n++) mbar_try(&s_full, it & 1);
   }
