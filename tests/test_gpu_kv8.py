@@ -274,6 +274,59 @@ def test_attend_many_short_sequences(n):
     check_attend(attend_state(rng, list(lens), list(np.minimum(lens, rng.integers(0, 3, n))), 2, 2, 32, "i8", "f32"))
 
 
+# Many rows a sequence: the tensor-core form (256 rows on average, head_dim 64 or 128, 16-bit rows).
+@pytest.mark.parametrize("fmt", ["e4m3", "i8"])
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+@pytest.mark.parametrize("Hq,H,D", [(8, 2, 64), (14, 2, 128), (4, 4, 64)])
+@pytest.mark.parametrize("rows,lens,window", [
+    ([130, 1, 300], [200, 64, 300], 0), ([257], [257], 0), ([300, 290], [900, 290], 70), ([256], [5000], 0)])
+def test_attend_many_rows(fmt, ty, Hq, H, D, rows, lens, window):
+    if Hq == 4:
+        rows, lens = [4 * r for r in rows], [max(4 * r, l) for r, l in zip(rows, lens)]
+    rng = np.random.default_rng(sum(rows) + D)
+    check_attend(attend_state(rng, lens, rows, Hq, H, D, fmt, ty, pad=2), window=window)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_many_rows_at_the_edges(D):
+    rng = np.random.default_rng(D)
+    # more rows than positions, no rows, nothing held, a refused sequence
+    s = attend_state(rng, [100, 50, 0, -1, 400], [300, 0, 20, 300, 400], 8, 2, D, "e4m3", "bf16", pad=5)
+    check_attend(s)
+    check_attend(s, scale=0.0)
+    check_attend(s, scale=-0.3, ld=8 * D + 8)
+    for i, n in enumerate(s["lens"]):  # codes behind the end
+        if n > 0 and n % 32:
+            s["codes"][s["table"][i, (n - 1) // 32], :, :, (n - 1) % 32 + 1:] = 0xFF
+    check_attend(s)
+    s["table"][4, 3], s["table"][4, 7], s["table"][0, 0] = -1, s["codes"].shape[0], 1 << 30
+    check_attend(s)
+    s["scales"][:, :, 1] *= (2.0 ** rng.integers(-40, 30, s["scales"].shape[:2])).astype(np.float32)
+    s["scales"][:, :, 1] *= 1.37
+    check_attend(s, window=90)
+
+
+def test_attend_many_rows_not_finite_scales():
+    rng = np.random.default_rng(15)
+    for which in (0, 1):
+        s = attend_state(rng, [300], [300], 2, 1, 64, "e4m3", "f16")
+        s["scales"][s["table"][0, 4], 0, which] = np.nan  # positions 128..159
+        got = call_attend(s)
+        assert np.isfinite(got[:128]).all() and np.isnan(got[128:]).all()
+        got = call_attend(s, window=20)
+        assert np.isnan(got[128:160]).all() and np.isfinite(got[179:]).all() and np.isfinite(got[:128]).all()
+
+
+def test_attend_many_rows_repeat_bit_for_bit_and_status():
+    rng = np.random.default_rng(16)
+    s = attend_state(rng, [3000, 700], [300, 512], 14, 2, 64, "e4m3", "bf16")
+    ws = smotor.Kv8Workspace()
+    a = call_attend(s, ws=ws)
+    for _ in range(3):
+        assert np.array_equal(call_attend(s, ws=ws), a)
+    ws.status(stream())
+
+
 def test_attend_rows_that_see_nothing():
     rng = np.random.default_rng(9)
     s = attend_state(rng, [0, -1, 2, 40], [1, 2, 4, 1], 4, 2, 64, "e4m3", "f32", pad=2)  # row count above the length
