@@ -51,14 +51,21 @@ struct Shape {
   static constexpr bool SPLIT = sizeof(T) == 4;
   static constexpr uint32_t WARPS = NR == 8 ? (SPLIT && HDV > 64 ? 12 : 16) : (HDV > 64 ? 12 : 16);
   static constexpr uint32_t VALUES = TILE * HDV, SCALES = 2 * VALUES;  // a page: K's codes, V's, then the scales
-  static constexpr uint32_t STAGE = SCALES + 16;
+  static constexpr uint32_t STAGE = SCALES + 128;
   // Byte offset of 16-byte column c of row r. The columns of each 128 bytes are exchanged by the row, so that
   // the 8 lanes of a shared-memory phase, (g, t) with two g for K and with four rows 2t for V, meet 8 of them.
   static __device__ uint32_t at(uint32_t r, uint32_t c) {
     if (HDV == 128) return r * 128 + ((c ^ ((r >> 1 & 3) << 1) ^ ((r & 1) << 2)) << 4);
     return (r >> 1) * 128 + ((((r & 1) << 2 | c) ^ ((r >> 1 & 3) << 1)) << 4);
   }
-  static constexpr uint32_t PART = NR * HDV * 4, ML = NR * 2 * 4;  // a partial result: o, then m and l
+  // The same for the accesses of a lane, from its first offset `base`: all others are constants away, with the
+  // column's bit 2 flipped (64 bytes; areas begin at multiples of 128) or not.
+  static __device__ uint32_t copy_at(uint32_t base, uint32_t i) { return (HDV == 128 && (i & 1) ? base ^ 64 : base) + i * 512; }
+  static __device__ uint32_t k_at(uint32_t base, uint32_t n, uint32_t sg) { return (sg ? base ^ 64 : base) + n * 8 * HDV; }
+  static __device__ uint32_t v_at(uint32_t base, uint32_t half, uint32_t i) {
+    return (i & 1 ? base ^ 64 : base) + half * 16 * HDV + (i >> 1) * 8 * HDV + (HDV == 128 ? (i & 1) * 128 : 0);
+  }
+  static constexpr uint32_t PART = NR * HDV * 4, ML = 128;  // a partial result: o, then m and l
   static constexpr uint32_t RING = STAGE > PART + ML ? STAGE : PART + ML;
   static constexpr uint32_t WARP = RING + PART + ML;  // the second partial lies over the page, done by then
   static constexpr uint32_t TOTAL = WARPS * WARP;
@@ -159,7 +166,7 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
   constexpr bool SPLIT = L::SPLIT;
   constexpr uint32_t WARPS = L::WARPS, THREADS = WARPS * 32;
   constexpr int MT = HDV / 16, SEG = HDV / 64, NB = NR / 8;  // M tiles of O^T, 64-dim segments, n tiles of rows
-  extern __shared__ float4 attn_smem4[];
+  extern __shared__ __align__(128) float4 attn_smem4[];
   __shared__ int64_t chunk_base[THREADS + 1];
   __shared__ int64_t warp_sum[WARPS];
   // A warp's partial results: of a unit that began before its share (0), of one that goes on behind it (1).
@@ -172,6 +179,9 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const uint32_t hd = FULL ? HDV : a.c.hd;
   const uint32_t ring = smem_addr(attn_smem4) + warp * L::WARP;
+  // Lane (g, t) reads K's rows g, g + 8, .. and V's rows 2t, 2t + 1, 2t + 8, ..
+  const uint32_t copy_base = ring + L::at(lane / (HDV / 16), lane % (HDV / 16)), k_base = ring + L::at(g, t);
+  const uint32_t v_base = ring + L::VALUES + (HDV == 128 ? L::at(2 * t, g) : L::at(2 * t, g >> 1) + (g & 1) * 8);
 
   // ---- the tile list: prefix sums over the sequences ----
   const uint32_t per_thread = (a.n_seqs + THREADS - 1) / THREADS;
@@ -197,10 +207,11 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
     __syncthreads();
   }
   const int64_t total = chunk_base[THREADS];
-  // Equal shares; at least two pages, so that a short list is not all merging.
-  const int64_t n_warps = (int64_t)gridDim.x * WARPS;
-  const int64_t share = max((total + n_warps - 1) / n_warps, (int64_t)2);
-  const int64_t x_begin = min(total, ((int64_t)blockIdx.x * WARPS + warp) * share), x_end = min(total, x_begin + share);
+  // Equal shares, a page more or less, of as many CTAs as have two pages a warp (a short list is not all merging).
+  const int64_t ctas = max(min((int64_t)gridDim.x, (total + 2 * WARPS - 1) / (2 * WARPS)), (int64_t)1), n_warps = ctas * WARPS;
+  auto share_begin = [&](int64_t w) { return min(w, n_warps) * total / n_warps; };
+  auto cta_of = [&](int64_t x) { return ((x + 1) * ctas - 1) / total; };  // the CTA whose share holds page x
+  const int64_t my_warp = (int64_t)blockIdx.x * WARPS + warp, x_begin = share_begin(my_warp), x_end = share_begin(my_warp + 1);
 
   if (!FULL) {  // columns behind hd stay zero
     for (uint32_t i = lane * 16; i < L::SCALES; i += 512)
@@ -262,8 +273,20 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
       };
       // K's or V's 32 rows of a page, 512 consecutive bytes a warp and step. Rows at and behind
       // `n` arrive as zeros: behind a sequence's end lies anything.
-      auto copy_rows = [&](uint32_t dst, const uint8_t* src, int32_t n) {
-        const uint32_t cpr = hd / 16;
+      auto copy_rows = [&](uint32_t area, const uint8_t* src, int32_t n) {
+        if constexpr (FULL) {
+          const uint32_t dst = copy_base + area;
+          src += lane * 16;
+          if (n >= (int32_t)KV8_PAGE) {
+#pragma unroll
+            for (uint32_t i = 0; i < HDV / 16; i++) copy16(L::copy_at(dst, i), src + i * 512, true);
+          } else {
+#pragma unroll
+            for (uint32_t i = 0; i < HDV / 16; i++) copy16(L::copy_at(dst, i), src + i * 512, (int32_t)((i * 32 + lane) / (HDV / 16)) < n);
+          }
+          return;
+        }
+        const uint32_t cpr = hd / 16, dst = ring + area;
 #pragma unroll
         for (uint32_t i = 0; i < HDV / 16; i++) {
           if (!FULL && i >= cpr) break;
@@ -274,14 +297,14 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
       auto fetch_k = [&](int32_t pg, uint32_t id) {  // an id outside the pool: no such page, its positions take no part
         if (pg < tile_stop && id < a.c.n_pages) {
           const uint64_t at = ((uint64_t)id * a.c.heads + head) * 2;
-          copy_rows(ring, a.c.codes + at * KV8_PAGE * hd, KV8_PAGE);
+          copy_rows(0, a.c.codes + at * KV8_PAGE * hd, KV8_PAGE);
           if (lane == 0) copy8(ring + L::SCALES, a.c.scales + at, true);
         }
         copy_commit();
       };
       auto fetch_v = [&](int32_t pg, uint32_t id) {
         if (pg < tile_stop && id < a.c.n_pages)
-          copy_rows(ring + L::VALUES, a.c.codes + (((uint64_t)id * a.c.heads + head) * 2 + 1) * KV8_PAGE * hd,
+          copy_rows(L::VALUES, a.c.codes + (((uint64_t)id * a.c.heads + head) * 2 + 1) * KV8_PAGE * hd,
                     sq.len - pg * (int32_t)TILE);
         copy_commit();
       };
@@ -365,7 +388,7 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
           for (int sg = 0; sg < SEG; sg++) {
             uint4 k[4];
 #pragma unroll
-            for (int n = 0; n < 4; n++) k[n] = lds16(ring + L::at(n * 8 + g, sg * 4 + t));
+            for (int n = 0; n < 4; n++) k[n] = lds16(L::k_at(k_base, n, sg));
 #pragma unroll
             for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -473,12 +496,11 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
             uint32_t vr[4][HDV / 32];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-              const uint32_t row = 16 * half + 2 * t + (i & 1) + 8 * (i >> 1);
               if constexpr (HDV == 128) {
-                const uint4 v = lds16(ring + L::VALUES + L::at(row, g));
+                const uint4 v = lds16(L::v_at(v_base, half, i));
                 vr[i][0] = v.x, vr[i][1] = v.y, vr[i][2] = v.z, vr[i][3] = v.w;
               } else {
-                const uint2 v = lds8(ring + L::VALUES + L::at(row, g >> 1) + (g & 1) * 8);
+                const uint2 v = lds8(L::v_at(v_base, half, i));
                 vr[i][0] = v.x, vr[i][1] = v.y;
               }
             }
@@ -568,14 +590,17 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
 
   // ---- units cut between warps ----
   // In warp order, slot 0 before slot 1, the pieces of a unit follow one another.
-  const int64_t cta_share = share * WARPS, cta_begin = (int64_t)blockIdx.x * cta_share, cta_end = cta_begin + cta_share;
+  const int64_t cta_begin = share_begin((int64_t)blockIdx.x * WARPS), cta_end = share_begin((int64_t)(blockIdx.x + 1) * WARPS);
   const int64_t mine = lane < WARPS * 2 ? piece[lane].unit : -1;
   const uint32_t there = __ballot_sync(~0u, mine >= 0);
   const uint32_t before = there & ((1u << lane) - 1);
   const int64_t previous = __shfl_sync(~0u, mine, before ? 31 - __clz(before) : 0);
   uint32_t starts = __ballot_sync(~0u, mine >= 0 && (!before || previous != mine));
   int32_t open[2] = {-1, -1};  // pieces of units that other CTAs share: begun before this one, and in it
-  while (starts) {
+  // Few units: all threads for each in turn; more (short ones): a warp for each.
+  const bool apart = __popc(starts) > 4;
+  const uint32_t first_item = apart ? lane : threadIdx.x, item_step = apart ? 32 : THREADS;
+  for (uint32_t nth = 0; starts; nth++) {
     const uint32_t i = __ffs(starts) - 1;
     starts &= starts - 1;
     const uint32_t ids = there & (starts ? (1u << (__ffs(starts) - 1)) - 1 : ~0u) & ~((1u << i) - 1);  // its pieces
@@ -584,7 +609,8 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
     const uint32_t side = pc.unit < cta_begin ? 0 : 1;
     float* gpart = a.part + ((uint64_t)blockIdx.x * 2 + side) * KV8_PART_FLOATS;
     if (!whole) open[side] = (int32_t)i;
-    for (uint32_t at = threadIdx.x; at < pc.rows * (HDV / 4); at += THREADS) {
+    if (apart && nth % WARPS != warp) continue;
+    for (uint32_t at = first_item; at < pc.rows * (HDV / 4); at += item_step) {
       const uint32_t row = at / (HDV / 4), d = at % (HDV / 4) * 4;
       float m = MINM, l = 0.f;
       float4 o = make_float4(0, 0, 0, 0);
@@ -613,8 +639,8 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
     uint32_t last = 0;
     if (open[threadIdx.x] >= 0) {
       const Piece& pc = piece[open[threadIdx.x]];
-      const int64_t c0 = pc.unit / cta_share;
-      const uint32_t others = (uint32_t)((pc.end - 1) / cta_share - c0);
+      const int64_t c0 = cta_of(pc.unit);
+      const uint32_t others = (uint32_t)(cta_of(pc.end - 1) - c0);
       last = atomicInc(a.cnt + c0, others) == others;
     }
     last_flag[threadIdx.x] = last;
@@ -624,8 +650,8 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
     if (last_flag[side]) {
       __threadfence();
       const Piece pc = piece[open[side]];
-      const int64_t c0 = pc.unit / cta_share;
-      const uint32_t others = (uint32_t)((pc.end - 1) / cta_share - c0);  // CTAs behind the first
+      const int64_t c0 = cta_of(pc.unit);
+      const uint32_t others = (uint32_t)(cta_of(pc.end - 1) - c0);  // CTAs behind the first
       auto part = [&](uint32_t c) { return a.part + ((uint64_t)(c0 + c) * 2 + (c ? 0 : 1)) * KV8_PART_FLOATS; };
       // Every (row, 4 dims) is summed by `ways` threads, each over every ways-th CTA, with
       // the loads of eight in flight; then over the ways, in order.

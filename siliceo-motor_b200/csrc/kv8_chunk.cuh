@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
   constexpr uint32_t GROUP8 = HD / 8 * 128;        // bytes of 8 positions: 16-byte columns of 8 rows each
   constexpr uint32_t OPERAND = CH_STEP / 8 * GROUP8;  // bytes of a step's K or V
   constexpr uint32_t ITEMS = CH_STEP * HD / 16 / 128;  // 16-code loads of a decode thread
-  extern __shared__ float4 attn_smem4[];
+  extern __shared__ __align__(128) float4 attn_smem4[];
   uint8_t* ops = reinterpret_cast<uint8_t*>(attn_smem4);  // K, K, V, V
   __shared__ int64_t chunk_base[CH_THREADS + 1];
   __shared__ int64_t warp_sum[CH_WARPS];
