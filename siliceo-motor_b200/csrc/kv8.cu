@@ -136,9 +136,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv8_plan_kernel(Kv8PlanArgs a) {
 //
 // Rows of a page that one call writes are consecutive (a "run": slots rise by
 // one inside a page). A CTA takes the runs that begin in its `chunk` rows, for
-// one head: 128 threads K, 128 V, eight elements a thread and pass, the whole
-// run in registers between its maximum and its encoding, so the rows are read
-// once. Memory-bound for prompts; for one row a sequence it is the chain
+// one head's K or V: eight elements a thread and pass, the whole run in
+// registers between its maximum and its encoding, so the rows are read once.
+// Memory-bound for prompts; for one row a sequence it is the chain
 // slots -> scale -> store.
 constexpr uint32_t APP_GROUP = 128;
 
@@ -210,27 +210,27 @@ __device__ uint32_t rescale4(uint32_t c, float ratio) {
 }
 
 template <uint32_t FMT, typename T>
-__global__ void __launch_bounds__(2 * APP_GROUP)
+__global__ void __launch_bounds__(APP_GROUP, sizeof(T) == 4 ? 8 : 10)
     kv8_append_kernel(Kv8 c, const T* k, const T* v, uint32_t n_rows, uint64_t ld_k, uint64_t ld_v, const int64_t* slots,
                       uint32_t chunk) {
-  __shared__ uint32_t tops[2][2][4];
-  const uint32_t lane = threadIdx.x & 31, which = threadIdx.x / APP_GROUP, tid = threadIdx.x % APP_GROUP, head = blockIdx.y;
+  __shared__ uint32_t tops[2][4];
+  const uint32_t lane = threadIdx.x & 31, tid = threadIdx.x, head = blockIdx.y >> 1, which = blockIdx.y & 1;
   const uint32_t base = blockIdx.x * chunk, cpr = c.hd / 8;
   const T* src = which ? v : k;
   const uint64_t ld = which ? ld_v : ld_k;
   const int64_t n_slots = (int64_t)c.n_pages * KV8_PAGE;
-  const uint32_t t_mine = base + lane;
-  bool begins = false;
-  if (lane < chunk && t_mine < n_rows) {
-    const int64_t s = slots[t_mine];
-    begins = s >= 0 && s < n_slots && (t_mine == 0 || s % KV8_PAGE == 0 || slots[t_mine - 1] != s - 1);
-  }
+  // the chunk's slots and those of the 32 rows behind it, where its last run may end: lane l has rows l and 32 + l
+  auto slot_of = [&](uint32_t t) { return t < n_rows ? slots[t] : -2; };
+  const int64_t s_lo = slot_of(base + lane), s_hi = slot_of(base + 32 + lane), s_first = base ? slots[base - 1] : -2;
+  const int64_t s_up = __shfl_up_sync(~0u, s_lo, 1), s_before = lane ? s_up : s_first;
+  const bool begins = lane < chunk && s_lo >= 0 && s_lo < n_slots && (s_lo % KV8_PAGE == 0 || s_before != s_lo - 1);
   uint32_t todo = __ballot_sync(~0u, begins), buf = 0;
   for (; todo; todo &= todo - 1, buf ^= 1) {
-    const uint32_t t0 = base + __ffs(todo) - 1;
-    const int64_t s0 = slots[t0];
+    const uint32_t first = __ffs(todo) - 1, t0 = base + first;
+    const int64_t s0 = __shfl_sync(~0u, s_lo, first);
     const uint32_t page = (uint32_t)(s0 / KV8_PAGE), off = (uint32_t)(s0 % KV8_PAGE);
-    const bool goes = off + lane < KV8_PAGE && t0 + lane < n_rows && slots[t0 + lane] == s0 + lane;
+    const int64_t a = __shfl_sync(~0u, s_lo, (first + lane) & 31), b = __shfl_sync(~0u, s_hi, (first + lane) & 31);
+    const bool goes = off + lane < KV8_PAGE && (first + lane < 32 ? a : b) == s0 + lane;
     const uint32_t stop = ~__ballot_sync(~0u, goes), rows = stop ? __ffs(stop) - 1 : 32;
     float* scale_at = c.scales + ((uint64_t)page * c.heads + head) * 2 + which;
     uint8_t* codes = c.codes + (((uint64_t)page * c.heads + head) * 2 + which) * KV8_PAGE * c.hd;
@@ -252,9 +252,9 @@ __global__ void __launch_bounds__(2 * APP_GROUP)
       for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
     }
     top = __reduce_max_sync(~0u, top);
-    if (lane == 0) tops[buf][which][tid / 32] = top;
-    asm volatile("bar.sync %0, %1;" ::"r"(which + 1), "n"(APP_GROUP) : "memory");
-    for (int i = 0; i < 4; i++) top = max(top, tops[buf][which][i]);
+    if (lane == 0) tops[buf][tid / 32] = top;
+    __syncthreads();
+    for (int i = 0; i < 4; i++) top = max(top, tops[buf][i]);
 
     // A row that is not finite makes the scale NaN: the page's values of this head are NaN from then on.
     const bool bad = top >= 0x7F800000u || old != old;
@@ -288,8 +288,8 @@ cudaError_t append_typed(const Kv8& c, const void* k, const void* v, uint32_t n_
                          const int64_t* slots, cudaStream_t st) {
   // Rows a CTA looks at: 32 (about one run) for prompts; fewer while that would leave SMs without work.
   const uint32_t chunk = std::max(1u, std::min(32u, (uint32_t)((uint64_t)n_rows * c.heads / 1024)));
-  const dim3 grid((n_rows + chunk - 1) / chunk, c.heads);
-  kv8_append_kernel<FMT, T><<<grid, 2 * APP_GROUP, 0, st>>>(c, (const T*)k, (const T*)v, n_rows, ld_k, ld_v, slots, chunk);
+  const dim3 grid((n_rows + chunk - 1) / chunk, c.heads * 2);
+  kv8_append_kernel<FMT, T><<<grid, APP_GROUP, 0, st>>>(c, (const T*)k, (const T*)v, n_rows, ld_k, ld_v, slots, chunk);
   return cudaGetLastError();
 }
 

@@ -43,6 +43,7 @@ namespace sm {
 namespace {
 
 constexpr uint32_t TILE = KV8_PAGE;  // positions of a step
+constexpr int32_t SHORT = 4;         // pages of a unit that is never cut: a merge would cost more
 constexpr float MINM = -1e30f;       // running maximum of a row that has seen nothing
 
 // Shape of a kernel. HD: head dims, at run time at most HDV. NR: rows of a unit.
@@ -242,7 +243,14 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
       const int64_t in_seq = x - seq_base;
       const int64_t unit = in_seq >> 31 ? in_seq / sq.tiles : (int64_t)((uint32_t)in_seq / (uint32_t)sq.tiles);
       const int64_t unit_base = seq_base + unit * sq.tiles, unit_end = unit_base + sq.tiles;
-      const int64_t stop = min(unit_end, x_end);
+      int64_t stop = min(unit_end, x_end);
+      if (sq.tiles <= SHORT) {  // not cut: the warp in whose share it begins does all of it
+        if (x > unit_base) {
+          x = unit_end;
+          continue;
+        }
+        stop = unit_end;
+      }
       const uint32_t block = (uint32_t)unit / a.c.heads, head = (uint32_t)unit - block * a.c.heads;
       const uint32_t total_rows = (uint32_t)sq.n_rows * a.group, row_base = block * NR;
       const uint32_t rows = min(NR, total_rows - row_base);
@@ -597,10 +605,8 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
   const int64_t previous = __shfl_sync(~0u, mine, before ? 31 - __clz(before) : 0);
   uint32_t starts = __ballot_sync(~0u, mine >= 0 && (!before || previous != mine));
   int32_t open[2] = {-1, -1};  // pieces of units that other CTAs share: begun before this one, and in it
-  // Few units: all threads for each in turn; more (short ones): a warp for each.
-  const bool apart = __popc(starts) > 4;
-  const uint32_t first_item = apart ? lane : threadIdx.x, item_step = apart ? 32 : THREADS;
-  for (uint32_t nth = 0; starts; nth++) {
+  uint32_t taken = 0;  // threads that the units so far occupy: the next unit's items go to those behind them
+  while (starts) {
     const uint32_t i = __ffs(starts) - 1;
     starts &= starts - 1;
     const uint32_t ids = there & (starts ? (1u << (__ffs(starts) - 1)) - 1 : ~0u) & ~((1u << i) - 1);  // its pieces
@@ -609,8 +615,9 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
     const uint32_t side = pc.unit < cta_begin ? 0 : 1;
     float* gpart = a.part + ((uint64_t)blockIdx.x * 2 + side) * KV8_PART_FLOATS;
     if (!whole) open[side] = (int32_t)i;
-    if (apart && nth % WARPS != warp) continue;
-    for (uint32_t at = first_item; at < pc.rows * (HDV / 4); at += item_step) {
+    const uint32_t items = pc.rows * (HDV / 4), first_item = threadIdx.x >= taken ? threadIdx.x - taken : threadIdx.x + THREADS - taken;
+    taken = (taken + items) % THREADS;
+    for (uint32_t at = first_item; at < items; at += THREADS) {
       const uint32_t row = at / (HDV / 4), d = at % (HDV / 4) * 4;
       float m = MINM, l = 0.f;
       float4 o = make_float4(0, 0, 0, 0);
