@@ -147,6 +147,13 @@ struct Vec8;
 template <>
 struct Vec8<float> {
   float4 a, b;
+  __device__ uint32_t top(uint32_t t) const {  // the larger of t and the magnitudes, as bits of a float
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; i++) t = max(t, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    return t;
+  }
+  static __device__ uint32_t wide(uint32_t t) { return t; }
   __device__ void get(float (&x)[8]) const {
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
   }
@@ -154,6 +161,15 @@ struct Vec8<float> {
 template <>
 struct Vec8<__half> {
   uint4 v;
+  // the larger of t and the magnitudes, two at a time as 16-bit integers (NaN above infinity)
+  __device__ uint32_t top(uint32_t t) const {
+    t = __vmaxu2(t, v.x & 0x7FFF7FFFu), t = __vmaxu2(t, v.y & 0x7FFF7FFFu);
+    return __vmaxu2(__vmaxu2(t, v.z & 0x7FFF7FFFu), v.w & 0x7FFF7FFFu);
+  }
+  static __device__ uint32_t wide(uint32_t t) {  // as bits of a float
+    t = max(t >> 16, t & 0xFFFFu);
+    return t >= 0x7C00u ? 0x7F800000u + (t > 0x7C00u) : __float_as_uint(__half2float(__ushort_as_half((unsigned short)t)));
+  }
   __device__ void get(float (&x)[8]) const {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     for (int i = 0; i < 4; i++) {
@@ -165,6 +181,12 @@ struct Vec8<__half> {
 template <>
 struct Vec8<__nv_bfloat16> {
   uint4 v;
+  // the larger of t and the magnitudes, two at a time as 16-bit integers (NaN above infinity)
+  __device__ uint32_t top(uint32_t t) const {
+    t = __vmaxu2(t, v.x & 0x7FFF7FFFu), t = __vmaxu2(t, v.y & 0x7FFF7FFFu);
+    return __vmaxu2(__vmaxu2(t, v.z & 0x7FFF7FFFu), v.w & 0x7FFF7FFFu);
+  }
+  static __device__ uint32_t wide(uint32_t t) { return max(t & 0xFFFF0000u, t << 16); }  // as bits of a float
   __device__ void get(float (&x)[8]) const {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     for (int i = 0; i < 4; i++) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
@@ -209,13 +231,16 @@ __device__ uint32_t rescale4(uint32_t c, float ratio) {
   return encode4<FMT>(x);
 }
 
-template <uint32_t FMT, typename T>
+// EVEN: head_dim divides 1024, a thread's vectors share a column.
+template <uint32_t FMT, typename T, bool EVEN>
 __global__ void __launch_bounds__(APP_GROUP, sizeof(T) == 4 ? 8 : 10)
     kv8_append_kernel(Kv8 c, const T* k, const T* v, uint32_t n_rows, uint64_t ld_k, uint64_t ld_v, const int64_t* slots,
                       uint32_t chunk) {
   __shared__ uint32_t tops[2][4];
   const uint32_t lane = threadIdx.x & 31, tid = threadIdx.x, head = blockIdx.y >> 1, which = blockIdx.y & 1;
   const uint32_t base = blockIdx.x * chunk, cpr = c.hd / 8;
+  const uint32_t row0 = tid / cpr, col0 = tid - row0 * cpr;
+  const uint32_t inv_cpr = (65536 + cpr - 1) / cpr;  // x * inv_cpr >> 16 is x / cpr for the x here (below 512)
   const T* src = which ? v : k;
   const uint64_t ld = which ? ld_v : ld_k;
   const int64_t n_slots = (int64_t)c.n_pages * KV8_PAGE;
@@ -236,33 +261,35 @@ __global__ void __launch_bounds__(APP_GROUP, sizeof(T) == 4 ? 8 : 10)
     uint8_t* codes = c.codes + (((uint64_t)page * c.heads + head) * 2 + which) * KV8_PAGE * c.hd;
     const float old = off ? *scale_at : 0.f;
 
+    // Vector i of this thread: 8 elements at column 8 col of row row(i), 128 vectors behind vector i - 1.
+    auto row = [&](uint32_t i) { return EVEN ? row0 + i * (APP_GROUP / cpr) : (tid + i * APP_GROUP) * inv_cpr >> 16; };
+    auto col = [&](uint32_t i) { return EVEN ? col0 : tid + i * APP_GROUP - row(i) * cpr; };
     Vec8<T> raw[4];
     uint32_t top = 0;
+    const T* from = src + (uint64_t)t0 * ld + head * c.hd;
 #pragma unroll
-    for (uint32_t i = 0; i < 4; i++) {
-      const uint32_t at = tid + i * APP_GROUP, row = at / cpr, col = at % cpr;
-      if (row < rows) raw[i] = *reinterpret_cast<const Vec8<T>*>(src + (uint64_t)(t0 + row) * ld + head * c.hd + col * 8);
-    }
+    for (uint32_t i = 0; i < 4; i++)
+      if (row(i) < rows) raw[i] = *reinterpret_cast<const Vec8<T>*>(from + (uint64_t)row(i) * ld + col(i) * 8);
 #pragma unroll
-    for (uint32_t i = 0; i < 4; i++) {
-      if ((tid + i * APP_GROUP) / cpr >= rows) continue;
-      float x[8];
-      raw[i].get(x);
-#pragma unroll
-      for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-    }
-    top = __reduce_max_sync(~0u, top);
+    for (uint32_t i = 0; i < 4; i++)
+      if (row(i) < rows) top = raw[i].top(top);
+    top = __reduce_max_sync(~0u, Vec8<T>::wide(top));
     if (lane == 0) tops[buf][tid / 32] = top;
     __syncthreads();
     for (int i = 0; i < 4; i++) top = max(top, tops[buf][i]);
 
+    uint8_t* to = codes + off * c.hd;
     // A row that is not finite makes the scale NaN: the page's values of this head are NaN from then on.
-    const bool bad = top >= 0x7F800000u || old != old;
-    const float need = page_scale<FMT>(min(top, 0x7F7FFFFFu));
-    const float s = bad ? __uint_as_float(0x7FC00000u) : fmaxf(old, need);
-    const float inv = bad ? 0.f : 1.f / s;
+    if (top >= 0x7F800000u || old != old) {
+      if (tid == 0) *scale_at = __uint_as_float(0x7FC00000u);
+#pragma unroll
+      for (uint32_t i = 0; i < 4; i++)
+        if (row(i) < rows) *reinterpret_cast<uint2*>(to + row(i) * c.hd + col(i) * 8) = make_uint2(0, 0);
+      continue;
+    }
+    const float s = fmaxf(old, page_scale<FMT>(top)), inv = 1.f / s;
     if (tid == 0) *scale_at = s;
-    if (!bad && off && s > old) {
+    if (off && s > old) {
       const float ratio = old * inv;
       for (uint32_t at = tid * 8; at < off * c.hd; at += APP_GROUP * 8) {
         uint2* p = reinterpret_cast<uint2*>(codes + at);
@@ -272,13 +299,12 @@ __global__ void __launch_bounds__(APP_GROUP, sizeof(T) == 4 ? 8 : 10)
     }
 #pragma unroll
     for (uint32_t i = 0; i < 4; i++) {
-      const uint32_t at = tid + i * APP_GROUP, row = at / cpr, col = at % cpr;
-      if (row >= rows) continue;
+      if (row(i) >= rows) continue;
       float x[8];
       raw[i].get(x);
 #pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = bad ? 0.f : x[j] * inv;
-      *reinterpret_cast<uint2*>(codes + (off + row) * c.hd + col * 8) = make_uint2(encode4<FMT>(x), encode4<FMT>(x + 4));
+      for (int j = 0; j < 8; j++) x[j] *= inv;
+      *reinterpret_cast<uint2*>(to + row(i) * c.hd + col(i) * 8) = make_uint2(encode4<FMT>(x), encode4<FMT>(x + 4));
     }
   }
 }
@@ -289,7 +315,8 @@ cudaError_t append_typed(const Kv8& c, const void* k, const void* v, uint32_t n_
   // Rows a CTA looks at: 32 (about one run) for prompts; fewer while that would leave SMs without work.
   const uint32_t chunk = std::max(1u, std::min(32u, (uint32_t)((uint64_t)n_rows * c.heads / 1024)));
   const dim3 grid((n_rows + chunk - 1) / chunk, c.heads * 2);
-  kv8_append_kernel<FMT, T><<<grid, APP_GROUP, 0, st>>>(c, (const T*)k, (const T*)v, n_rows, ld_k, ld_v, slots, chunk);
+  auto* kern = 1024 % c.hd ? kv8_append_kernel<FMT, T, false> : kv8_append_kernel<FMT, T, true>;
+  kern<<<grid, APP_GROUP, 0, st>>>(c, (const T*)k, (const T*)v, n_rows, ld_k, ld_v, slots, chunk);
   return cudaGetLastError();
 }
 
