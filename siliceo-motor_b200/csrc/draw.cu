@@ -73,6 +73,7 @@ struct alignas(16) Shared {
   uint64_t post[10];                // what this CTA tells the others; no slot is written again before all have read it
   uint64_t cut;                     // rank 0's answer
   uint64_t found_run;
+  double anchor;
   uint32_t n_cand, found[2], n_here, n_left, at_zero;
 };
 
@@ -546,64 +547,90 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
           sum += m[j];
           var += m[j] * m[j];
         }
-        double run = block_before(sum, sh.warp64b, &all), var_all;
+        const double before_m = block_before(sum, sh.warp64b, &all);
+        double var_all;
         block_before(var, sh.warp64, &var_all);
+        // The bin in which the guessed sums pass `want` (sh.found[which]; ~0: none).
+        auto guess = [&](double want, int which) {
+          double run = before_m;
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            if (run < want && run + m[j] >= want) sh.found[which] = 4 * tid + j;
+            run += m[j];
+          }
+        };
         // A bin's values are off its middle by RANGE / BINS / sqrt(12), all alike where they are few distinct
         // ones (16-bit logits). Errors of hundreds of bins cancel, and those before and behind the border partly
         // do: 0.4 of the standard deviation leaves a few bins, and held in every one of 480 simulated rows.
         const double want = round ? (goal - (double)above) / UNIT : (double)p.top_p * all;
         const double slack = 0.4 * RANGE / BINS / 3.46 * sqrt(var_all) + 3e-5 * all;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          if (run < want - slack && run + m[j] >= want - slack) sh.found[0] = 4 * tid + j;
-          if (run < want + slack && run + m[j] >= want + slack) sh.found[1] = 4 * tid + j;
-          run += m[j];
-        }
+        guess(want - slack, 0);
+        guess(want + slack, 1);
         __syncthreads();
-        // Exact masses of a range to try; it then holds the border, or what lies on one side of it does.
-        // The first is the guess, later ones halves: the range shrinks every turn.
+        // Exact masses of a range of bins to try: it then holds the border, or what lies on one side of it does,
+        // so the range that may hold it, [bin_a, bin_b], shrinks every turn. The first turn tries the guess, the
+        // later ones a guess from the exact mass before bin_a, which is a few bins off at most. Where all values
+        // are in [lo, hi] a thread looks at consecutive ones, as in the draw, keeps its mass before bin_a (`mine`)
+        // and collects the range's places: the draw then needs no pass of its own.
         uint32_t try_a = sh.found[0] == ~0u ? 0 : sh.found[0], try_b = sh.found[1] == ~0u ? BINS - 1 : max(sh.found[1], try_a);
+        mine = 0;
         for (int turn = 0;; turn++) {
-          uint64_t ma = 0, mi = 0, ml = 0;
-          if (everything && !turn) {
-            // Consecutive values, as in the draw, and the range's places collected on the way: the draw then
-            // needs no pass of its own.
-            const float fa = (float)try_a, fb = try_b == BINS - 1 ? INFINITY : (float)(try_b + 1);
+          uint64_t ma = 0, mi = 0, ml = 0;  // in the bins from bin_a to try_a, of the range, behind it (first turn)
+          if (everything) {
+            const float f0 = (float)bin_a, fa = (float)try_a, fb = try_b == BINS - 1 ? INFINITY : (float)(try_b + 1);
             if (tid == 0) sh.n_here = 0;
             __syncthreads();
-            for (uint32_t i = i0; i < i1; i += 4) {
-              float x[4];
-              uint64_t w[4];
+            auto collect = [&](float x, uint32_t i) {
+              const uint32_t at = atomicAdd(&sh.n_here, 1u);
+              if (at < CAP) local[at] = place(x, begin + i);
+            };
+            if (!turn) {
+              for (uint32_t i = i0; i < i1; i += 4) {
+                float x[4];
+                uint64_t w[4];
 #pragma unroll
-              for (int j = 0; j < 4; j++) x[j] = i + j < i1 ? value(vals[i + j]) : -INFINITY;
+                for (int j = 0; j < 4; j++) x[j] = i + j < i1 ? value(vals[i + j]) : -INFINITY;
 #pragma unroll
-              for (int j = 0; j < 4; j++) w[j] = wt.of(x[j]);
+                for (int j = 0; j < 4; j++) w[j] = wt.of(x[j]);
 #pragma unroll
-              for (int j = 0; j < 4; j++) {
-                const float b = fast_bin(x[j]);
-                ml += w[j];
-                ma += b < fa ? w[j] : 0;
-                if (b >= fa && b < fb) {
-                  mi += w[j];
-                  const uint32_t at = atomicAdd(&sh.n_here, 1u);
-                  if (at < CAP) local[at] = place(x[j], begin + i + j);
+                for (int j = 0; j < 4; j++) {
+                  const float b = fast_bin(x[j]);
+                  ml += w[j];
+                  ma += b < fa ? w[j] : 0;
+                  if (b >= fa && b < fb) {
+                    mi += w[j];
+                    collect(x[j], i + j);
+                  }
+                }
+              }
+              ml -= ma + mi;
+            } else {
+#pragma unroll 4
+              for (uint32_t i = i0; i < i1; i++) {
+                const float x = value(vals[i]), b = fast_bin(x);
+                if (!(b >= f0 && b < fb)) continue;
+                const uint64_t w = wt.of(x);
+                if (b < fa) {
+                  ma += w;
+                } else {
+                  mi += w;
+                  collect(x, i);
                 }
               }
             }
-            ml -= ma + mi;
-            mine = ma;
           } else {
             each([&](float x, uint32_t i) {
               const uint64_t pl = place(x, begin + i);
               if (!(x > -INFINITY) || pl < lo || pl > hi) return;
               const uint32_t b = bin_of(x, pl);
-              if (turn ? b < try_a || b > try_b : round && b > try_b) return;
+              if (b < bin_a || (b > try_b && (round || turn))) return;
               const uint64_t w = wt.of(x);
               if (b < try_a) ma += w;
               else if (b <= try_b) mi += w;
               else ml += w;
             });
           }
+          const uint64_t ma_here = ma, mi_here = mi;
           ma = block_sum(ma, sh.warp64);
           mi = block_sum(mi, sh.warp64b);
           ml = block_sum(ml, sh.warp64);
@@ -611,18 +638,40 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
           if (tid == 0) sh.post[slot] = ma, sh.post[slot + 1] = mi, sh.post[slot + 2] = ml;
           cl.sync();
           uint64_t unused;
-          ma = add_up(slot, unused), mi = add_up(slot + 1, unused), ml = add_up(slot + 2, unused);
-          if (turn) ma = mass_above;  // try_a is bin_a
+          ma = mass_above + add_up(slot, unused), mi = add_up(slot + 1, unused), ml = add_up(slot + 2, unused);
           if (!round && !turn) goal = (double)p.top_p * (double)(ma + mi + ml);
           const bool begins = try_a == bin_a || above + ma == 0 || (double)(above + ma) < goal;
           const bool ends = try_b == bin_b || (double)(above + ma + mi) >= goal;
-          if (begins && ends) bin_a = try_a, bin_b = try_b, mass_above = ma;
-          else if (!begins) bin_b = try_a - 1;
-          else bin_a = try_b + 1, mass_above = ma + mi;
+          if (begins && ends) {
+            bin_a = try_a, bin_b = try_b, mass_above = ma;
+            mine += ma_here;
+          } else if (!begins) {
+            bin_b = try_a - 1;
+          } else {
+            bin_a = try_b + 1, mass_above = ma + mi;
+            mine += ma_here + mi_here;
+          }
           count_range();
-          direct = everything && !turn && bin_a == try_a && bin_b == try_b && n_in <= CAP;
-          if (n_in <= CAP || bin_a == bin_b) break;
-          try_a = bin_a, try_b = (bin_a + bin_b) / 2;
+          direct = everything && begins && ends && n_in <= CAP;
+          if (direct || (!everything && n_in <= CAP) || (bin_a == bin_b && n_in > CAP)) break;
+          // the next range: all that is left, if that is few; else the bin of the new guess and its neighbours
+          try_a = bin_a, try_b = bin_b;
+          if (n_in <= CAP) continue;
+          if (tid == 0) sh.found[0] = (bin_a + bin_b) / 2;
+          __syncthreads();
+          if (4 * tid <= bin_a && bin_a < 4 * tid + 4) {
+            double run = before_m;
+#pragma unroll
+            for (int j = 0; j < 4; j++) run += 4 * tid + j < bin_a ? m[j] : 0.0;
+            sh.anchor = run;
+          }
+          __syncthreads();
+          guess(sh.anchor + (goal - (double)above - (double)mass_above) / UNIT, 0);
+          __syncthreads();
+          const uint32_t t = min(max(sh.found[0], bin_a), bin_b);
+          __syncthreads();
+          if (bin_b - bin_a > 2) try_a = max(bin_a, t ? t - 1 : 0), try_b = min(bin_b, t + 1);
+          else try_a = try_b = t;
         }
       }
       const bool small = !mass && round == 0 && n_above + n_in <= CAP;  // all the top_k at once
