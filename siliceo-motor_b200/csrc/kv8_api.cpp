@@ -163,17 +163,24 @@ int sm_kv8_ws_new(sm_kv8_ws** out) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return cuda_error("sm_kv8_ws_new", e);
+    // One allocation, the counters and the error word behind the partial results. They are zeroed on a stream of
+    // the call's own, so that no other work is waited for.
+    const size_t part = kv8_attn_part_floats((uint32_t)sms) * sizeof(float);
+    const size_t cnt = (kv8_attn_counters((uint32_t)sms) + 1) * sizeof(uint32_t);
     auto* w = new sm_kv8_ws;
     w->device = dev;
     w->sms = (uint32_t)sms;
-    const size_t cnt = (kv8_attn_counters(w->sms) + 1) * sizeof(uint32_t);
-    e = cudaMalloc(&w->part, kv8_attn_part_floats(w->sms) * sizeof(float));
-    if (e == cudaSuccess) e = cudaMalloc(&w->cnt, cnt);
-    if (e == cudaSuccess) e = cudaMemset(w->cnt, 0, cnt);
-    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    cudaStream_t st = nullptr;
+    e = cudaMalloc(&w->part, part + cnt);
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+    if (e == cudaSuccess) {
+      w->cnt = (uint32_t*)((char*)w->part + part);
+      e = cudaMemsetAsync(w->cnt, 0, cnt, st);
+      if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+      cudaStreamDestroy(st);
+    }
     if (e != cudaSuccess) {
       cudaFree(w->part);
-      cudaFree(w->cnt);
       delete w;
       return cuda_error("sm_kv8_ws_new", e);
     }
@@ -188,7 +195,6 @@ int sm_kv8_ws_free(sm_kv8_ws* w) {
   cudaGetDevice(&dev);
   if (dev != w->device) cudaSetDevice(w->device);
   cudaFree(w->part);
-  cudaFree(w->cnt);
   if (dev != w->device) cudaSetDevice(dev);
   delete w;
   return SM_OK;

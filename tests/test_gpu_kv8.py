@@ -388,6 +388,74 @@ def test_attend_repeats_bit_for_bit_and_on_another_stream():
         assert np.array_equal(call_attend(s, ws=ws), a)
 
 
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+def test_attend_one_kv_head_for_many(ty):
+    rng = np.random.default_rng(17)
+    check_attend(attend_state(rng, [40, 100, 1], [1, 2, 1], 40, 1, 64, "e4m3", ty))
+
+
+def test_attend_thousands_of_sequences():
+    rng = np.random.default_rng(18)
+    lens = rng.integers(0, 4, 5000)
+    check_attend(attend_state(rng, list(lens), [1] * 5000, 1, 1, 16, "i8", "f32"))
+
+
+def test_attend_two_calls_at_once():
+    rng = np.random.default_rng(19)
+    states = [attend_state(rng, [6000, 200], [1, 1], 14, 2, 64, "e4m3", "f32"),
+              attend_state(rng, [900, 700], [300, 300], 8, 2, 128, "i8", "bf16")]
+    d, want, q, out, cache, ws = [], [], [], [], [], []
+    for s in states:
+        want.append(call_attend(s))
+        d.append({k: dev(s[k]) for k in ("codes", "scales", "table", "first", "lens")})
+        q.append(s["q"].cuda().contiguous())
+        out.append(torch.zeros_like(q[-1]))
+        P, H, _, _, D = s["codes"].shape
+        cache.append(smotor.Kv8Cache(d[-1]["codes"].data_ptr(), d[-1]["scales"].data_ptr(), P, H, D, FMT[s["fmt"]]))
+        ws.append(smotor.Kv8Workspace())
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for i, s in enumerate(states):
+            T, Hq, _ = s["q"].shape
+            cache[i].attend(ws[i], q[i].data_ptr(), out[i].data_ptr(), TYPES[s["ty"]][1], T, Hq, 2, d[i]["lens"].data_ptr(),
+                            d[i]["first"].data_ptr(), d[i]["table"].data_ptr(), s["table"].shape[1],
+                            stream=streams[i].cuda_stream)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert np.array_equal(out[i].double().cpu().numpy(), want[i])
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_pages_behind_four_gigabytes(many):
+    """The same rows through low and through high pages of a pool of 4.5 GB."""
+    rng = np.random.default_rng(20)
+    P, D, n = 560000, 128, 300
+    codes = torch.empty((P, 1, 2, 32, D), dtype=torch.uint8, device="cuda")
+    scales = torch.ones((P, 1, 2), device="cuda")
+    cache = smotor.Kv8Cache(codes.data_ptr(), scales.data_ptr(), P, 1, D)
+    k, v = (dev(rng.normal(0, 1, (n, 1, D)), torch.bfloat16) for _ in range(2))
+    rows = n if many else 1
+    q = dev(rng.normal(0, 1, (rows, 2, D)), torch.bfloat16)
+    lens, first = dev(np.array([n], np.int32)), dev(np.array([0, rows], np.int32))
+    ws, got = smotor.Kv8Workspace(), []
+    for base in (0, P - 10):
+        pages = np.arange(base, base + 10)
+        slots = dev((pages[np.arange(n) // 32] * 32 + np.arange(n) % 32).astype(np.int64))
+        table, out = dev(pages.astype(np.int32)), torch.zeros_like(q)
+        cache.append(k.data_ptr(), v.data_ptr(), smotor.BF16, n, slots.data_ptr(), stream=stream())
+        cache.attend(ws, q.data_ptr(), out.data_ptr(), smotor.BF16, rows, 2, 1, lens.data_ptr(), first.data_ptr(),
+                     table.data_ptr(), 10, stream=stream())
+        torch.cuda.synchronize()
+        got.append((codes[base:base + 10].cpu(), scales[base:base + 10].cpu(), out.float().cpu()))
+    used = np.arange(320).reshape(10, 32) < n
+    for a, b in zip(got[0], got[1]):
+        if a.dtype == torch.uint8:
+            a, b = (x[:, 0].transpose(1, 2)[torch.from_numpy(used)] for x in (a, b))
+        assert torch.equal(a, b)
+    assert bool(torch.isfinite(got[0][2]).all()) and float(got[0][2].abs().max()) > 0
+
+
 def test_device_refusals():
     host = torch.zeros(4096, pin_memory=True)
     on = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda").data_ptr()
