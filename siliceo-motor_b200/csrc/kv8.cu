@@ -18,7 +18,8 @@ namespace {
 // the end of the free list. So every CTA makes both prefix sums of all the
 // sequences itself (a few KB out of L2) and then works on rows of its own:
 // one launch, no CTA waits for another. What it costs is latency (a dozen
-// dependent steps), not bytes.
+// dependent steps), not bytes: 4.2 us a launch for 32 sequences, 5.6 us for
+// 512 sequences with 33 thousand rows (0.55 MB).
 constexpr uint32_t PLAN_THREADS = 512;
 constexpr uint32_t PLAN_ROWS = 1024;  // rows a CTA takes at a time
 
@@ -138,8 +139,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv8_plan_kernel(Kv8PlanArgs a) {
 // one inside a page). A CTA takes the runs that begin in its `chunk` rows, for
 // one head's K or V: eight elements a thread and pass, the whole run in
 // registers between its maximum and its encoding, so the rows are read once.
-// Memory-bound for prompts; for one row a sequence it is the chain
-// slots -> scale -> store.
+// Memory-bound for prompts: 24 prompts of up to 1999 f16 rows, 8 heads of 128,
+// to e4m3 in 40 us (224 MB, 5.5 TB/s, 0.85 of the measured 6515 GB/s; 47 us
+// while the magnitudes were compared one by one). For one row a sequence it is
+// the chain slots -> scale -> store: 2.5 us for 32 rows.
 constexpr uint32_t APP_GROUP = 128;
 
 template <typename T>

@@ -26,6 +26,13 @@
 // error word and an abort flag, after which the other waits return at once,
 // the CTA waits (bounded) for the MMAs it issued, frees its tensor memory and
 // leaves.
+//
+// Measured on B200: 2 sequences, chunks of up to 1024 rows over up to 8192
+// positions, 28/4 heads of 128, bf16 rows: 349 us, 462 TFLOP/s of what the rows
+// see (0.28 of the measured 1679); the streaming form takes 800. A step takes
+// a CTA about 4000 cycles, and its chain S - weights - P V bounds it: scores
+// from tensor memory twice with 72 registers a thread (two CTAs an SM), about
+// 1800; the two products with their barriers, about 2000.
 #pragma once
 #include "kv8_attn.cuh"
 #include "tc_common.cuh"
