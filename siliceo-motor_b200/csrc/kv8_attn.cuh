@@ -532,11 +532,19 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
               }
 #pragma unroll
               for (int nb = 0; nb < NB; nb++) {
-                mma(o[nb][2 * j2], lo, pf[nb][half][0], pf[nb][half][1]);
-                mma(o[nb][2 * j2 + 1], hi, pf[nb][half][0], pf[nb][half][1]);
                 if constexpr (SPLIT) {
-                  mma(o[nb][2 * j2], lo, pf[nb][half][2], pf[nb][half][3]);
-                  mma(o[nb][2 * j2 + 1], hi, pf[nb][half][2], pf[nb][half][3]);
+                  // The tensor core cuts its sums off: over thousands of positions that bias passes 22 bits. So
+                  // f32 rows' products of 16 positions are added to O in f32, rounded.
+                  float x[2][4] = {};
+                  mma(x[0], lo, pf[nb][half][2], pf[nb][half][3]);
+                  mma(x[0], lo, pf[nb][half][0], pf[nb][half][1]);
+                  mma(x[1], hi, pf[nb][half][2], pf[nb][half][3]);
+                  mma(x[1], hi, pf[nb][half][0], pf[nb][half][1]);
+#pragma unroll
+                  for (int i = 0; i < 4; i++) o[nb][2 * j2][i] += x[0][i], o[nb][2 * j2 + 1][i] += x[1][i];
+                } else {
+                  mma(o[nb][2 * j2], lo, pf[nb][half][0], pf[nb][half][1]);
+                  mma(o[nb][2 * j2 + 1], hi, pf[nb][half][0], pf[nb][half][1]);
                 }
               }
             }

@@ -400,6 +400,18 @@ def test_attend_thousands_of_sequences():
     check_attend(attend_state(rng, list(lens), [1] * 5000, 1, 1, 16, "i8", "f32"))
 
 
+@pytest.mark.parametrize("fmt,D", [("e4m3", 128), ("i8", 32)])
+def test_attend_f32_keeps_its_bits_over_thousands_of_positions(fmt, D):
+    """The 2-norm of the error: 6400 positions are 400 sums of 16, each rounded to 2^-24 of what is there: as a
+    random walk 20 x 2^-24 = 1.2e-6; scores off by |t| 2^-23 ln2, |t| < 10, 0.8e-6; the rest is smaller. A sum
+    cut off instead of rounded would be 400 x 2^-24 = 2.4e-5 low."""
+    rng = np.random.default_rng(22)
+    s = attend_state(rng, [6400, 6399], [40, 8], 4, 1, D, fmt, "f32")
+    got = call_attend(s)
+    want, _ = ref.attend(s["codes"], s["scales"], fmt, s["q"].double().numpy(), s["lens"], s["first"], s["table"], D**-0.5)
+    assert np.linalg.norm(got - want) <= 4e-6 * np.linalg.norm(want)
+
+
 def test_attend_two_calls_at_once():
     rng = np.random.default_rng(19)
     states = [attend_state(rng, [6000, 200], [1, 1], 14, 2, 64, "e4m3", "f32"),
