@@ -9,7 +9,9 @@
 // w_j = 2^(t_j + e_j - m + 13), are then relative to the largest
 // *contribution* and fit f16 whatever the spread of the pages' scales, while
 // the denominator adds w_j 2^-e_j in f32. m is kept a whole number, so moving
-// it multiplies by a power of two and rounds nothing.
+// it multiplies by a power of two and rounds nothing. e_j is held to -60 .. 126,
+// so that 2^-e_j and sums of it stay in f32's range: smaller scales' weights
+// come out smaller instead.
 //
 // Bound by the cache bytes (2 hd a position and head): a warp copies a page at
 // a time into shared memory of its own, the next page's K under this page's
@@ -54,7 +56,7 @@ namespace {
 
 constexpr uint32_t TILE = KV8_PAGE;  // positions of a step
 constexpr int32_t SHORT = 4;         // pages of a unit that is never cut: a merge would cost more
-constexpr float MINM = -1e30f;       // running maximum of a row that has seen nothing
+constexpr float MINM = -3e38f;       // running maximum of a row that has seen nothing
 
 // Shape of a kernel. HD: head dims, at run time at most HDV. NR: rows of a unit.
 template <typename T, uint32_t HDV, uint32_t NR>
@@ -430,35 +432,34 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
           // ---- weights: s[nb][half][2 i + r] is position 16 half + 8 i + g, row 2t + r ----
           const float sk = __uint_as_float(sc.x), sv = __uint_as_float(sc.y);
           const int ev = min(max((int)(sc.y >> 23 & 255) - 127, -60), 126);
-          const float e = (float)ev, back = __uint_as_float((uint32_t)(127 - ev) << 23), frac = sv * back;
+          // the weights' factor 2^13 comes with the scale's fraction and goes into l as well
+          const float e = (float)ev, back = __uint_as_float((uint32_t)(127 + 13 - ev) << 23), frac = sv * back;
           const int32_t p0 = tile * (int32_t)TILE;
           const bool masked = p0 < all_lo || p0 + (int32_t)TILE > all_hi;
           float f[NB][2];
 #pragma unroll
           for (int nb = 0; nb < NB; nb++) f[nb][0] = mult[nb][0] * sk, f[nb][1] = mult[nb][1] * sk;
-          if (masked) {
-            // Unseen scores are -inf, whatever the codes there were; the factor, which may be
-            // zero, negative or NaN, is applied here and does not touch them again.
+          // u = t + e, rounded here and then only compared and subtracted: no weight passes 2^13 however large
+          // the scores are. Unseen ones are -inf, whatever the codes there were.
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++)
+          for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-              for (int k = 0; k < 8; k++) {
+            for (int k = 0; k < 8; k++) {
+              float& v = s[nb][k >> 2][k & 3];
+              v = fmaf(v, f[nb][k & 1], e);
+              if (masked) {
                 const int32_t pos = p0 + (int32_t)g + 8 * (k >> 1), last = last_pos[nb][k & 1];
-                float& v = s[nb][k >> 2][k & 3];
-                v = pos > last || (int64_t)pos <= last - w64 ? -INFINITY : v * f[nb][k & 1];
+                if (pos > last || (int64_t)pos <= last - w64) v = -INFINITY;
               }
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) f[nb][0] = f[nb][1] = 1.f;
-          }
+            }
           float top[NB][2];
           bool more = false;
 #pragma unroll
           for (int nb = 0; nb < NB; nb++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-              top[nb][r] = fmaxf(fmaxf(s[nb][0][r] * f[nb][r], s[nb][0][2 + r] * f[nb][r]),
-                                 fmaxf(s[nb][1][r] * f[nb][r], s[nb][1][2 + r] * f[nb][r]));
-              more |= top[nb][r] + e > m[nb][r];
+              top[nb][r] = fmaxf(fmaxf(s[nb][0][r], s[nb][0][2 + r]), fmaxf(s[nb][1][r], s[nb][1][2 + r]));
+              more |= top[nb][r] > m[nb][r];
             }
           if (__any_sync(~0u, more)) {
 #pragma unroll
@@ -469,8 +470,8 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
                 x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
                 x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
                 x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
-                // whole: e - m below is exact, and so is every factor between two maxima
-                const float mn = fmaxf(m[nb][r], ceilf(x + e)), alpha = ex2(m[nb][r] - mn);
+                // whole: every factor between two maxima is exact
+                const float mn = fmaxf(m[nb][r], ceilf(x)), alpha = ex2(m[nb][r] - mn);
                 m[nb][r] = mn;
                 l[nb][r] *= alpha;
 #pragma unroll
@@ -479,14 +480,13 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
           }
 #pragma unroll
           for (int nb = 0; nb < NB; nb++) {
-            const float c[2] = {e - m[nb][0] + 13.f, e - m[nb][1] + 13.f};
             float sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int half = 0; half < 2; half++) {
               float w[4];
 #pragma unroll
               for (int i = 0; i < 4; i++) {
-                const float y = ex2(fmaf(s[nb][half][i], f[nb][i & 1], c[i & 1]));
+                const float y = ex2(s[nb][half][i] - m[nb][i & 1]);
                 sum[i & 1] += y;
                 w[i] = y * frac;
                 if (masked && s[nb][half][i] == -INFINITY) w[i] = 0.f;  // frac may be NaN

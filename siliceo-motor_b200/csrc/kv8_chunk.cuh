@@ -387,7 +387,8 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
           for (int h = 0; h < 2; h++) {
             const float4 sc = scales[it & 3][h];
             const int ev = min(max((int)(__float_as_uint(sc.y) >> 23 & 255) - 127, -60), 126);
-            e[h] = (float)ev, back[h] = __uint_as_float((uint32_t)(127 - ev) << 23), frac[h] = sc.y * back[h];
+            // the weights' factor 2^12 comes with the scale's fraction and goes into l as well
+            e[h] = (float)ev, back[h] = __uint_as_float((uint32_t)(127 + 12 - ev) << 23), frac[h] = sc.y * back[h];
             f[h] = mult * sc.x;
             here[h] = sc.z != 0.f;
             masked |= !here[h];
@@ -413,13 +414,13 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
 #pragma unroll
               for (int i = 0; i < 32; i++)
                 x = fmaxf(x, !with_mask.value || (i >= lo[h] && i < hi[h]) ? __uint_as_float(s[i]) : -INFINITY);
-              if (x > -INFINITY) top = fmaxf(top, x * f[h] + e[h]);
+              if (x > -INFINITY) top = fmaxf(top, fmaf(x, f[h], e[h]));
             }
           };
           if (masked) largest(std::true_type{}); else largest(std::false_type{});
           // Weights up to 2^14 fit f16 (times a scale's fraction): the maximum may lag by a factor 4.
-          if (__any_sync(~0u, top > m + 2.f)) {
-            const float mn = top > m + 2.f ? ceilf(top) : m, alpha = ex2(m - mn);
+          if (__any_sync(~0u, top - m > 2.f)) {
+            const float mn = top - m > 2.f ? ceilf(top) : m, alpha = ex2(m - mn);
             m = mn;
             l *= alpha;
             if (step != pc.step) {
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
           auto weigh = [&](auto with_mask) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-              const float c = e[h] - m + 12.f;
+              const float c = e[h] - m;  // exact where it is used
               float sum = 0.f;
 #pragma unroll
               for (int half = 0; half < 2; half++) {
@@ -451,7 +452,9 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
                   for (int j = 0; j < 2; j++) {
                     const int col = 16 * half + 2 * i + j;
                     const bool see = !with_mask.value || (col >= lo[h] && col < hi[h]);
-                    y[j] = ex2(fmaf(__uint_as_float(s[2 * i + j]), f[h], c));
+                    // large scores: t + e rounded as for the maximum, so that no weight passes 2^14
+                    if (with_mask.value) y[j] = ex2(fmaf(__uint_as_float(s[2 * i + j]), f[h], e[h]) - m);
+                    else y[j] = ex2(fmaf(__uint_as_float(s[2 * i + j]), f[h], c));
                     if (!see) y[j] = 0.f;
                     sum += y[j];
                     y[j] = see ? y[j] * frac[h] : 0.f;  // frac may be NaN
@@ -463,7 +466,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
               l = fmaf(sum, back[h], l);
             }
           };
-          if (masked) weigh(std::true_type{}); else weigh(std::false_type{});
+          if (__any_sync(~0u, masked || fabsf(m) > 4194304.f)) weigh(std::true_type{}); else weigh(std::false_type{});
           tmem_wait_st();
           tc_fence_before();
           ch_arrive(&p_full);

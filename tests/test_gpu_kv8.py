@@ -16,6 +16,10 @@ errors of weights scale with) and to the output itself:
 draw: tokens equal; log probabilities to 2^-23 relative + 2e-7 (one rounding
 to f32 of a value computed in f64 from weights off by 2^-44 each).
 """
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -410,6 +414,89 @@ def test_attend_f32_keeps_its_bits_over_thousands_of_positions(fmt, D):
     got = call_attend(s)
     want, _ = ref.attend(s["codes"], s["scales"], fmt, s["q"].double().numpy(), s["lens"], s["first"], s["table"], D**-0.5)
     assert np.linalg.norm(got - want) <= 4e-6 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("ty,rows", [("f32", 3), ("bf16", 1), ("f16", 20), ("bf16", 300)])
+@pytest.mark.parametrize("size", [1e9, 1e31])
+def test_attend_of_huge_scores(ty, rows, size):
+    """Scores so large that one position has all the weight, in steps of f32 wider than the exponents the weights
+    are made of: the output is that position's V, rounded once."""
+    if ty == "f16":
+        size = 6e4 if size < 1e20 else 3e4
+    rng = np.random.default_rng(23)
+    s = attend_state(rng, [700, 90 + rows], [rows, rows], 4, 1, 64, "e4m3", ty)
+    s["q"] = (s["q"].float() * size).clamp(-3e38, 3e38).to(s["q"].dtype) if ty != "f16" else (s["q"].float() * size / 8).to(s["q"].dtype)
+    scale = 1e5 if ty == "f16" else 1.0
+    q = s["q"].double().numpy()
+    want, mag = ref.attend(s["codes"], s["scales"], "e4m3", q, s["lens"], s["first"], s["table"], scale)
+    got = call_attend(s, scale=scale)
+    assert np.all(np.isfinite(got))
+    # rows whose two best scores differ by less than rounding moves them are left out: K is known, so look at it
+    clear = leading(s, q) > 1e-5
+    assert clear.mean() > 0.9
+    half = {"f32": 2.0**-24, "f16": 2.0**-11, "bf16": 2.0**-8}[ty]
+    err = np.abs(got - want) - half * np.abs(want) - (2.0**-11 + 2e-5 if ty != "f32" else 2e-5) * np.abs(mag)
+    assert np.all(err[clear] <= 0)
+
+
+def leading(s, q):
+    """By how much each row's best score leads its second, relative to the largest one."""
+    K = ref.E4M3[s["codes"][:, 0, 0].astype(int)] * s["scales"][:, 0, 0].astype(np.float64)[:, None, None]
+    out = np.zeros(q.shape[:2])
+    for i, n in enumerate(s["lens"]):
+        r0, r1 = s["first"][i], s["first"][i + 1]
+        k = K[s["table"][i, :-(-n // 32)]].reshape(-1, q.shape[2])
+        for r in range(r0, r1):
+            t = np.sort(q[r] @ k[: n - (r1 - r0) + (r - r0) + 1].T, 1)
+            out[r] = (t[:, -1] - t[:, -2]) / np.abs(t).max(1) if t.shape[1] > 1 else 1.0
+    return out
+
+
+@pytest.mark.parametrize("ty,D,rows", [("f32", 16, 1), ("bf16", 128, 1), ("f16", 64, 7), ("bf16", 128, 400)])
+def test_attend_in_place_and_into_columns_beside_q(ty, D, rows):
+    rng = np.random.default_rng(24)
+    s = attend_state(rng, [3000, 17 + rows], [rows, rows], 4, 2, D, "i8", ty)
+    want = call_attend(s)
+    d = {k: dev(s[k]) for k in ("codes", "scales", "table", "first", "lens")}
+    cache, ws = smotor.Kv8Cache(d["codes"].data_ptr(), d["scales"].data_ptr(), len(s["codes"]), 2, D, smotor.KV8_I8), smotor.Kv8Workspace()
+    both = torch.full((2 * rows, 2, 4, D), 5.0, dtype=TYPES[ty][0], device="cuda")
+    both[:, 1] = s["q"].cuda()
+    q = s["q"].cuda().contiguous()
+    for x, y, ld in ((q.data_ptr(), q.data_ptr(), 0), (both[:, 1].data_ptr(), both.data_ptr(), 8 * D)):
+        cache.attend(ws, x, y, TYPES[ty][1], 2 * rows, 4, 2, d["lens"].data_ptr(), d["first"].data_ptr(),
+                     d["table"].data_ptr(), s["table"].shape[1], ld_q=ld, ld_out=ld, stream=stream())
+    torch.cuda.synchronize()
+    assert np.array_equal(q.double().cpu().numpy(), want) and np.array_equal(both[:, 0].double().cpu().numpy(), want)
+    assert torch.equal(both[:, 1].cpu(), s["q"])
+
+
+def test_first_calls_of_a_process_are_captured():
+    code = """
+import torch, smotor
+P = lambda *s, dt=torch.int32: torch.zeros(s, dtype=dt, device="cuda")
+ws = smotor.Kv8Workspace()
+codes, scales, q = P(4, 1, 2, 32, 64, dt=torch.uint8), P(4, 1, 2, dt=torch.float32), P(300, 4, 64, dt=torch.bfloat16)
+kv, out = q[:, :1].contiguous() + 1, q + 7
+lens, add, table, free, n_free = P(1), P(1) + 40, P(1, 4) - 1, P(4) + torch.arange(4, device="cuda", dtype=torch.int32), P(1) + 4
+lens_out, first, slots, status = P(1), P(2), P(300, dt=torch.int64), P(2)
+logits, par, u, tok = P(1, 100000, dt=torch.float32), torch.tensor([[1.0, 0, 0.9, 0]], device="cuda"), P(1, dt=torch.float32), P(1)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    s = torch.cuda.current_stream().cuda_stream
+    c = smotor.Kv8Cache(codes.data_ptr(), scales.data_ptr(), 4, 1, 64)
+    smotor.kv_plan(1, lens.data_ptr(), add.data_ptr(), table.data_ptr(), 4, free.data_ptr(), n_free.data_ptr(), 300,
+                   lens_out.data_ptr(), first.data_ptr(), slots.data_ptr(), status.data_ptr(), stream=s)
+    c.append(kv.data_ptr(), kv.data_ptr(), smotor.BF16, 300, slots.data_ptr(), stream=s)
+    for n in (300, 40):
+        c.attend(ws, q.data_ptr(), out.data_ptr(), smotor.BF16, n, 4, 1, lens_out.data_ptr(), first.data_ptr(),
+                 table.data_ptr(), 4, stream=s)
+    smotor.draw(logits.data_ptr(), smotor.F32, 1, 100000, par.data_ptr(), u.data_ptr(), tok.data_ptr(), stream=s)
+g.replay()
+torch.cuda.synchronize()
+assert bool((out[:40] == 1).all()) and bool((out[40:] == 7).all()) and int(tok[0]) == 0 and int(status[0]) == 2
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=os.path.dirname(smotor.__path__[0]))
 
 
 def test_attend_two_calls_at_once():
