@@ -364,13 +364,14 @@ typedef struct {
  *   entry is negative). pos_dev, seq_dev [n_rows] (each may be NULL): the
  *   row's position in its sequence (-1 like slots) and its sequence (-1 for a
  *   padding row).
- * - lens_out_dev [n_seqs] (not lens_dev itself): the new length, or -1 if the
+ * - lens_out_dev [n_seqs]: the new length, or -1 if the
  *   sequence is refused: its length or add is negative, it would exceed its
  *   table row or n_rows, or it needs pages and the pages that it and the
  *   sequences before it need are more than the list has. A refused sequence
  *   keeps its place in first_dev (a negative add counts as 0), takes no page,
  *   and its lens_out of -1 makes its rows attend to nothing.
- * - status_dev [2]: pages left in the free list, number of refused sequences. */
+ * - status_dev [2]: pages left in the free list, number of refused sequences.
+ * No output may share bytes with another argument (n_free_dev included). */
 int sm_kv_plan(uint64_t n_seqs, const int32_t* lens_dev, const int32_t* add_dev, int32_t* table_dev, uint64_t table_ld,
                const int32_t* free_dev, const int32_t* n_free_dev, uint64_t n_rows, int32_t* lens_out_dev,
                int32_t* first_dev, int64_t* slots_dev, int32_t* pos_dev, int32_t* seq_dev, int32_t* status_dev,
@@ -415,8 +416,10 @@ int sm_kv8_ws_status(const sm_kv8_ws* w, void* stream);
  * row that sees nothing (a length of 0 or -1 among them) gets zeros, and rows
  * behind first_dev[n_seqs] are left as they were. Positions whose page id is
  * not in the pool take no part. Scales may be any finite values >= 0.
+ * out may be q itself (with q's stride), or other columns of one matrix.
  * Products and sums are f32; scores and weights enter the tensor cores with
- * 22 bits for F32 rows and as f16 for F16 and BF16 rows. */
+ * 22 bits for F32 rows and as f16 for F16 and BF16 rows. V scales below 2^-60
+ * lose bits of them. */
 int sm_kv8_attend(const sm_kv8* c, sm_kv8_ws* ws, const void* q_dev, void* out_dev, uint32_t type, uint64_t n_rows,
                   uint32_t n_heads, uint64_t ld_q, uint64_t ld_out, uint64_t n_seqs, const int32_t* lens_dev,
                   const int32_t* first_dev, const int32_t* table_dev, uint64_t table_ld, float scale, uint32_t window,
@@ -439,6 +442,7 @@ typedef struct {
  * gets token -1 and log probability -inf. logprobs_dev (may be NULL): natural
  * log of the token's probability among the kept ones (0 when greedy). Weights
  * are summed exactly in 64 bits: a draw does not depend on the order of sums.
+ * Outputs may not share bytes with other arguments.
  * Not sm_sample: that one reproduces the reference's f32 sampler and its RNG
  * bit for bit, on host logits. */
 int sm_draw(const void* logits_dev, uint32_t type, uint64_t n_rows, uint64_t ld, uint64_t vocab, const uint8_t* mask_dev,

@@ -33,23 +33,31 @@ int cuda_error(const char* fn, cudaError_t e) {
   return e == cudaErrorMemoryAllocation ? SM_ERR_OOM : SM_ERR_CUDA;
 }
 
-// The checks of one call, the first failure kept: conditions, null and
-// misaligned pointers as they are named, and in memory(), which needs a
-// device, that each pointer is memory of the current one.
+// The checks of one call, the first failure kept: conditions; null and
+// misaligned pointers as they are named; outputs that share bytes with another
+// argument (its CTAs read inputs after others have written); and in memory(),
+// which needs a device, that each pointer is memory of the current one.
 struct Check {
   const char* fn;
   int dev = -1, rc = SM_OK;
-  struct { const char* name; const void* p; } ptrs[12];
+  struct { const char* name; const void* p; uint64_t bytes; bool out; } ptrs[13];
   uint32_t n_ptrs = 0;
   explicit Check(const char* f) : fn(f) {}
   void want(bool ok, const char* what) {
     if (!rc && !ok) rc = arg_error(fn, what);
   }
-  void ptr(const char* name, const void* p, size_t align, bool optional = false) {
+  // bytes 0: not compared with the others
+  void ptr(const char* name, const void* p, size_t align, bool optional = false, uint64_t bytes = 0, bool out = false) {
     if (rc || (!p && optional)) return;
     if (!p) { rc = arg_error(fn, std::string(name) + " is null"); return; }
     if ((uintptr_t)p % align) { rc = arg_error(fn, std::string(name) + " must be " + std::to_string(align) + "-byte aligned"); return; }
-    ptrs[n_ptrs++] = {name, p};
+    for (uint32_t i = 0; i < n_ptrs; i++)
+      if (bytes && ptrs[i].bytes && (out || ptrs[i].out) && (uintptr_t)p < (uintptr_t)ptrs[i].p + ptrs[i].bytes &&
+          (uintptr_t)ptrs[i].p < (uintptr_t)p + bytes) {
+        rc = arg_error(fn, std::string(name) + " overlaps " + ptrs[i].name);
+        return;
+      }
+    ptrs[n_ptrs++] = {name, p, bytes, out};
   }
   int memory() {
     if (rc) return rc;
@@ -111,18 +119,18 @@ int sm_kv_plan(uint64_t n_seqs, const int32_t* lens_dev, const int32_t* add_dev,
     ck.want(n_seqs <= KV8_PLAN_MAX_SEQS, "at most 16384 sequences");
     ck.want(n_rows <= 0x7FFFFFFF, "at most 2^31 - 1 rows");
     ck.want(table_ld <= 0x7FFFFFFF, "table_ld must be below 2^31");
-    ck.want(!n_seqs || lens_out_dev != lens_dev, "lens_out_dev must not be lens_dev");
-    ck.ptr("lens_dev", lens_dev, 4, !n_seqs);
-    ck.ptr("add_dev", add_dev, 4, !n_seqs);
-    ck.ptr("table_dev", table_dev, 4, !n_seqs || !table_ld);
-    ck.ptr("free_dev", free_dev, 4, true);
-    ck.ptr("n_free_dev", n_free_dev, 4);
-    ck.ptr("lens_out_dev", lens_out_dev, 4, !n_seqs);
-    ck.ptr("first_dev", first_dev, 4);
-    ck.ptr("slots_dev", slots_dev, 8, !n_rows);
-    ck.ptr("pos_dev", pos_dev, 4, true);
-    ck.ptr("seq_dev", seq_dev, 4, true);
-    ck.ptr("status_dev", status_dev, 4);
+    if (ck.rc) return ck.rc;
+    ck.ptr("lens_dev", lens_dev, 4, !n_seqs, n_seqs * 4);
+    ck.ptr("add_dev", add_dev, 4, !n_seqs, n_seqs * 4);
+    ck.ptr("table_dev", table_dev, 4, !n_seqs || !table_ld, n_seqs * table_ld * 4, true);
+    ck.ptr("free_dev", free_dev, 4, true, 4);  // its length lies on the device
+    ck.ptr("n_free_dev", n_free_dev, 4, false, 4);
+    ck.ptr("lens_out_dev", lens_out_dev, 4, !n_seqs, n_seqs * 4, true);
+    ck.ptr("first_dev", first_dev, 4, false, (n_seqs + 1) * 4, true);
+    ck.ptr("slots_dev", slots_dev, 8, !n_rows, n_rows * 8, true);
+    ck.ptr("pos_dev", pos_dev, 4, true, n_rows * 4, true);
+    ck.ptr("seq_dev", seq_dev, 4, true, n_rows * 4, true);
+    ck.ptr("status_dev", status_dev, 4, false, 8, true);
     if (ck.memory()) return ck.rc;
     Kv8PlanArgs a{lens_dev, add_dev, table_dev, table_ld, free_dev, n_free_dev, (uint32_t)n_seqs, (uint32_t)n_rows,
                   lens_out_dev, first_dev, slots_dev, pos_dev, seq_dev, status_dev};
@@ -237,6 +245,14 @@ int sm_kv8_attend(const sm_kv8* c, sm_kv8_ws* ws, const void* q_dev, void* out_d
     ck.want(ld_q >= width && ld_out >= width && ld_q < (1ull << 32) && ld_out < (1ull << 32), "a row stride is below n_heads x head_dim, or 2^32 and above");
     ck.want(ld_q * es % 16 == 0 && ld_out * es % 16 == 0, "row strides must be multiples of 16 bytes");
     check_cache_memory(ck, c);
+    // Every row of q is read before it is written in out: they may be the same rows, or other columns of a matrix
+    // that holds both, but must not overlap in another way.
+    const uint64_t q0 = (uint64_t)(uintptr_t)q_dev, o0 = (uint64_t)(uintptr_t)out_dev, row = width * es;
+    const uint64_t q1 = q0 + ((n_rows - 1) * ld_q + width) * es, o1 = o0 + ((n_rows - 1) * ld_out + width) * es;
+    if (q0 < o1 && o0 < q1) {
+      const uint64_t pitch = ld_q * es, apart = (o0 > q0 ? o0 - q0 : q0 - o0) % pitch;
+      ck.want(ld_q == ld_out && (q0 == o0 || (apart >= row && apart <= pitch - row)), "out overlaps q other than row on row");
+    }
     ck.ptr("q_dev", q_dev, 16);
     ck.ptr("out_dev", out_dev, 16);
     ck.ptr("lens_dev", lens_dev, 4);
@@ -264,15 +280,16 @@ int sm_draw(const void* logits_dev, uint32_t type, uint64_t n_rows, uint64_t ld,
     const size_t es = type_size(type);
     ck.want(es, "type must be F32, F16 or BF16");
     ck.want(vocab >= 1 && vocab <= DRAW_MAX_VOCAB, "vocab must be 1..524288");
-    ck.want(!ld || ld >= vocab, "ld is below vocab");
+    ck.want(!ld || (ld >= vocab && ld < (1ull << 32)), "ld is below vocab, or 2^32 and above");
     ck.want(n_rows <= 65536, "at most 65536 rows");
     if (ck.rc || !n_rows) return ck.rc;
-    ck.ptr("logits_dev", logits_dev, es);
-    ck.ptr("mask_dev", mask_dev, 1, true);
-    ck.ptr("params_dev", params_dev, 16);
-    ck.ptr("u_dev", u_dev, 4);
-    ck.ptr("tokens_dev", tokens_dev, 4);
-    ck.ptr("logprobs_dev", logprobs_dev, 4, true);
+    const uint64_t span = ld && n_rows > 1 ? (n_rows - 1) * ld + vocab : n_rows * vocab;
+    ck.ptr("logits_dev", logits_dev, es, false, span * es);
+    ck.ptr("mask_dev", mask_dev, 1, true, span);
+    ck.ptr("params_dev", params_dev, 16, false, n_rows * sizeof(sm_draw_params));
+    ck.ptr("u_dev", u_dev, 4, false, n_rows * 4);
+    ck.ptr("tokens_dev", tokens_dev, 4, false, n_rows * 4, true);
+    ck.ptr("logprobs_dev", logprobs_dev, 4, true, n_rows * 4, true);
     if (ck.memory()) return ck.rc;
     static_assert(sizeof(sm_draw_params) == sizeof(DrawParams) && sizeof(DrawParams) == 16, "16 bytes a row");
     DrawArgs a{logits_dev, mask_dev, (const DrawParams*)params_dev, u_dev, tokens_dev, logprobs_dev, ld ? ld : vocab,

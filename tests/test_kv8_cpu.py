@@ -59,6 +59,57 @@ def test_append_of_no_rows_is_nothing():
     cache().append(0, 0, smotor.F32, 0, 0)
 
 
+class OneWorkspace:
+    h = C.create_string_buffer(64)  # read as device 0; the refusals come before
+
+
+# sm_kv_plan reads its inputs again after other CTAs have written; sm_draw likewise
+A = 1 << 20
+PLAN = dict(n_seqs=40, lens=A, add=2 * A, table=3 * A, table_ld=4, free=4 * A, n_free=5 * A, n_rows=50, lens_out=6 * A,
+            first=7 * A, slots=8 * A, pos=9 * A, seq=10 * A, status=11 * A)
+
+
+@pytest.mark.parametrize("out,other", [
+    ("lens_out", "lens"), ("lens_out", "add"), ("status", "n_free"), ("first", "add"), ("slots", "lens"), ("pos", "seq"),
+    ("seq", "slots"), ("table", "lens"), ("table", "free"), ("status", "first"), ("lens_out", "first")])
+@pytest.mark.parametrize("shift", [0, 8, -8])
+def test_plan_refuses_outputs_over_other_arguments(out, other, shift):
+    if shift == 8 and other in ("n_free", "free"):
+        shift = 0  # one entry of them is looked at
+    if shift == -8 and out == "status":
+        shift = -4
+    with pytest.raises(smotor.EngineError, match="overlaps") as e:
+        smotor.kv_plan(**{**PLAN, out: PLAN[other] + shift})
+    assert e.value.status == ARG
+
+
+@pytest.mark.parametrize("shift", [160, -160])
+def test_plan_takes_neighbours(shift):
+    with pytest.raises(smotor.EngineError) as e:  # not the refusal: there is no such memory
+        smotor.kv_plan(**{**PLAN, "lens_out": PLAN["lens"] + shift})
+    assert "overlaps" not in str(e.value)
+
+
+@pytest.mark.parametrize("kw,ok", [
+    (dict(out=A), True), (dict(out=A, ld_q=1024, ld_out=512), False), (dict(out=A + 16), False), (dict(out=A - 512), False),
+    (dict(out=A + 1024, ld_q=1024, ld_out=1024), True), (dict(out=A + 1024 + 2048, ld_q=1024, ld_out=1024), True),
+    (dict(out=A - 1024, ld_q=1024, ld_out=1024), True), (dict(out=A + 4096 + 16, ld_q=1024, ld_out=1024), False),
+    (dict(out=A + 1008, ld_q=1024, ld_out=1024), False), (dict(out=A + 9 * 1024), True)])
+def test_attend_refuses_rows_that_overlap_otherwise(kw, ok):
+    """9 f32 rows of 4 heads of 64: 1024 bytes each."""
+    a = dict(q=A, dtype=smotor.F32, n_rows=9, n_heads=4, n_seqs=1, lens=4 * A, first=5 * A, table=6 * A, table_ld=1)
+    with pytest.raises(smotor.EngineError) as e:  # where it takes them: there is no such memory
+        cache().attend(OneWorkspace, **{**a, **kw})
+    assert ("overlaps" in str(e.value)) == (not ok)
+
+
+@pytest.mark.parametrize("kw", [dict(tokens=3 * A), dict(tokens=2 * A + 32), dict(tokens=A + 396), dict(logprobs=5 * A + 4),
+                                dict(logprobs=4 * A - 4), dict(ld=1 << 32), dict(tokens=4 * A, ld=128, mask=4 * A - 1123)])
+def test_draw_refuses_outputs_over_other_arguments(kw):
+    a = dict(logits=A, dtype=smotor.F32, n_rows=9, vocab=100, params=2 * A, u=3 * A, tokens=5 * A, mask=4 * A)
+    refused(lambda: smotor.draw(**{**a, **kw}))
+
+
 class NoWorkspace:
     h = None
 
