@@ -28,11 +28,13 @@
 // leaves.
 //
 // Measured on B200: 2 sequences, chunks of up to 1024 rows over up to 8192
-// positions, 28/4 heads of 128, bf16 rows: 349 us, 462 TFLOP/s of what the rows
+// positions, 28/4 heads of 128, bf16 rows: 340 us, 474 TFLOP/s of what the rows
 // see (0.28 of the measured 1679); the streaming form takes 800. A step takes
-// a CTA about 4000 cycles, and its chain S - weights - P V bounds it: scores
-// from tensor memory twice with 72 registers a thread (two CTAs an SM), about
-// 1800; the two products with their barriers, about 2000.
+// an SM about 2200 cycles. The L1's data path is busy for 0.7 of them (scores
+// from tensor memory twice, weights back, operands written and read, codes),
+// the issue slots for 0.48, the tensor pipe for 0.2. A second S, its product
+// issued before the last step's weights are ready, with Q in shared memory,
+// hides the first product and still takes 364 us: the chain is not the bound.
 #pragma once
 #include "kv8_attn.cuh"
 #include "tc_common.cuh"
@@ -140,7 +142,8 @@ struct ChunkWalk {
 
 template <uint32_t FMT, typename T, uint32_t HD>
 __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnArgs a) {
-  constexpr uint32_t GROUP8 = HD / 8 * 128;        // bytes of 8 positions: 16-byte columns of 8 rows each
+  constexpr uint32_t CORE = 128 + 16;          // 16-byte columns of 8 rows, and a gap: see the decode warps
+  constexpr uint32_t GROUP8 = HD / 8 * CORE;   // bytes of 8 positions
   constexpr uint32_t OPERAND = CH_STEP / 8 * GROUP8;  // bytes of a step's K or V
   constexpr uint32_t ITEMS = CH_STEP * HD / 16 / 128;  // 16-code loads of a decode thread
   extern __shared__ __align__(128) float4 attn_smem4[];
@@ -217,8 +220,11 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
     const uint32_t tid = threadIdx.x % 128, is_v = warp >= CH_SOFT + CH_DEC / 2;
     uint64_t *full = is_v ? full_v : full_k, *empty = is_v ? empty_v : empty_k;
     uint8_t* dst = ops + is_v * 2 * OPERAND;
-    // An item is 16 codes of a row; a thread's are 128 apart, 8 rows side by side in a warp.
-    const uint32_t row0 = (tid & 7) + (tid >> 3) / (HD / 16) * 8, col = (tid >> 3) % (HD / 16);
+    // An item is 16 codes of a row; a thread's are 128 apart. A warp's 32 are 512 consecutive bytes, and the eight
+    // lanes of a shared-memory phase hold four columns of two rows: with 144 bytes a column pair's step they meet
+    // different banks (128 bytes would want eight rows a phase, whose loads take eight lines: 348 against 341 us).
+    const uint32_t col = HD == 128 ? (lane & 3) | (lane >> 1 & 4) : lane & 3;
+    const uint32_t row0 = HD == 128 ? tid / 32 * 4 + (lane >> 2 & 1) + (lane >> 4) * 2 : tid / 4;
     constexpr uint32_t ROWS = 128 / (HD / 16);  // rows between items
     const uint64_t src0 = ((uint64_t)is_v * KV8_PAGE + row0) * HD + col * 16;
     struct Ids { uint32_t id[2]; };  // a step's pages
@@ -251,12 +257,12 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
       if (is_v) ch_bar(3, 128); else ch_bar(2, 128);
 #pragma unroll
       for (uint32_t k = 0; k < ITEMS; k++) {
-        uint8_t* at = dst + st * OPERAND + (row0 + k * ROWS) / 8 * GROUP8 + col * 256 + row0 % 8 * 16;
+        uint8_t* at = dst + st * OPERAND + (row0 + k * ROWS) / 8 * GROUP8 + col * 2 * CORE + row0 % 8 * 16;
         uint4 lo, hi;
         decode4<FMT>(r[k].x, lo.x, lo.y), decode4<FMT>(r[k].y, lo.z, lo.w);
         decode4<FMT>(r[k].z, hi.x, hi.y), decode4<FMT>(r[k].w, hi.z, hi.w);
         *reinterpret_cast<uint4*>(at) = lo;
-        *reinterpret_cast<uint4*>(at + 128) = hi;
+        *reinterpret_cast<uint4*>(at + CORE) = hi;
       }
       if (brings) {
         // The slot's last readers, the softmax of step it - 4, are done: K's buffer came free after the scores
@@ -290,9 +296,9 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
   } else if (warp == CH_WARPS - 1) {
     // ------------------------------------------------ MMAs: the warp as one, an elected lane issues
     const uint32_t s_desc = umma_idesc_f16(CH_ROWS, CH_STEP), o_desc = umma_idesc_f16(CH_ROWS, HD) | 1u << 16;  // B N-major
-    const uint64_t k_base = umma_desc_k(smem_u32(ops), 128, GROUP8);
-    // N-major B: 8 positions x 8 dims are 128 bytes; groups of dims follow one another, groups of positions are GROUP8 apart
-    const uint64_t v_base = umma_desc_k(smem_u32(ops + 2 * OPERAND), GROUP8, 128);
+    const uint64_t k_base = umma_desc_k(smem_u32(ops), CORE, GROUP8);
+    // N-major B: 8 positions x 8 dims are 128 bytes, CORE apart; groups of dims follow one another, groups of positions are GROUP8 apart
+    const uint64_t v_base = umma_desc_k(smem_u32(ops + 2 * OPERAND), GROUP8, CORE);
     bool gone = false;
     while (walk.next(a, pc) && !gone) {
       if (pc.step >= pc.stop) continue;
@@ -307,7 +313,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
         const uint64_t kd = k_base + st * (OPERAND >> 4), vd = v_base + st * (OPERAND >> 4);
         if (ch_elect()) {
 #pragma unroll
-          for (uint32_t k = 0; k < HD / 16; k++) umma_ts(tb + CH_TS, tb + CH_TQ + 8 * k, kd + k * (256 >> 4), s_desc, k != 0);
+          for (uint32_t k = 0; k < HD / 16; k++) umma_ts(tb + CH_TS, tb + CH_TQ + 8 * k, kd + k * (2 * CORE >> 4), s_desc, k != 0);
           umma_commit(&s_full);
           umma_commit(&empty_k[st]);
         }
@@ -603,7 +609,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
 
 template <uint32_t FMT, typename T, uint32_t HD>
 cudaError_t chunk_launch(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) {
-  constexpr uint32_t smem = 4 * CH_STEP * HD * 2;
+  constexpr uint32_t smem = 4 * CH_STEP * HD * 2 / 128 * (128 + 16);  // four operands of columns CORE apart
   auto* kern = kv8_chunk_kernel<FMT, T, HD>;
   static SmemOnce once;
   const cudaError_t e = once.allow((const void*)kern, (int)smem);
@@ -613,7 +619,7 @@ cudaError_t chunk_launch(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) {
 }
 
 // Rows of a sequence, on average, from which this form is taken: 4 sequences of 4096 positions, 8 KV heads, take
-// 54 us in the streaming form and 72 us in this one with 112 rows each, 108 us and 94 us with 300.
+// 54 us in the streaming form and 72 us in this one with 112 rows each, 108 us and 90 us with 300.
 constexpr uint32_t CHUNK_MIN_ROWS = 256;
 template <typename T>
 bool chunk_takes(const Kv8AttnArgs& a) {
