@@ -35,9 +35,9 @@
 // shared memory, one cut between CTAs by the last of them to arrive.
 //
 // Measured on B200 (GPU time, launches back to back): 4 sequences of up to
-// 131072 positions, 28/4 heads of 128, bf16 rows, int8 codes: 80 us for 422 MB
-// (5.3 TB/s, 0.81 of the measured 6515 GB/s); 32 sequences of up to 4096, 32/8
-// heads: 46 us for 204 MB. The difference of the two is 6.4 TB/s, what is left
+// 131072 positions, 28/4 heads of 128, bf16 rows, int8 codes: 81 us for 422 MB
+// (5.2 TB/s, 0.80 of the measured 6515 GB/s); 32 sequences of up to 4096, 32/8
+// heads: 47 us for 204 MB. The difference of the two is 6.4 TB/s, what is left
 // is about 15 us a launch: 3 us to the first copies, 2 to 5 to the first codes,
 // 5 to 9 of merging and of SMs that finish at different times. Row blocks of
 // up to 8 rows keep 16 warps an SM (128 registers); 16 rows 12 warps. Without
