@@ -28,8 +28,8 @@
 // leaves.
 //
 // Measured on B200: 2 sequences, chunks of up to 1024 rows over up to 8192
-// positions, 28/4 heads of 128, bf16 rows: 340 us, 474 TFLOP/s of what the rows
-// see (0.28 of the measured 1679); the streaming form takes 800. A step takes
+// positions, 28/4 heads of 128, bf16 rows: 336 us, 480 TFLOP/s of what the rows
+// see (0.29 of the measured 1679); the streaming form takes 800. A step takes
 // an SM about 2200 cycles. The L1's data path is busy for 0.7 of them (scores
 // from tensor memory twice, weights back, operands written and read, codes),
 // the issue slots for 0.48, the tensor pipe for 0.2. A second S, its product
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
             e[h] = (float)ev, back[h] = __uint_as_float((uint32_t)(127 + 12 - ev) << 23), frac[h] = sc.y * back[h];
             f[h] = mult * sc.x;
             here[h] = sc.z != 0.f;
-            masked |= !here[h];
+            masked |= !here[h] || !(frac[h] >= 4096.f && frac[h] < 8192.f);
           }
           // columns of this row that it sees: [lo, hi) of each page's 32
           int32_t lo[2] = {0, 0}, hi[2] = {32, 32};
@@ -444,7 +444,9 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
           auto weigh = [&](auto with_mask) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-              const float c = e[h] - m;  // exact where it is used
+              // Unmasked: the factor goes into the exponent (exact for a power of two; else off by 2^-16 at most, as
+              // |m| is at most 256) and out of l again (336 us; multiplying each weight 340).
+              const float c = e[h] - m + __log2f(frac[h]), lb = with_mask.value ? back[h] : __fdividef(back[h], frac[h]);
               float sum = 0.f;
 #pragma unroll
               for (int half = 0; half < 2; half++) {
@@ -463,16 +465,16 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
                     else y[j] = ex2(fmaf(__uint_as_float(s[2 * i + j]), f[h], c));
                     if (!see) y[j] = 0.f;
                     sum += y[j];
-                    y[j] = see ? y[j] * frac[h] : 0.f;  // frac may be NaN
+                    if (with_mask.value) y[j] = see ? y[j] * frac[h] : 0.f;  // frac may be NaN
                   }
                   p[i] = pack_half(y[0], y[1]);
                 }
                 tmem_st8(tl + CH_TS + 16 * h + 8 * half, p);  // over columns already read
               }
-              l = fmaf(sum, back[h], l);
+              l = fmaf(sum, lb, l);
             }
           };
-          if (__any_sync(~0u, masked || fabsf(m) > 4194304.f)) weigh(std::true_type{}); else weigh(std::false_type{});
+          if (__any_sync(~0u, masked || fabsf(m) > 256.f)) weigh(std::true_type{}); else weigh(std::false_type{});
           tmem_wait_st();
           tc_fence_before();
           ch_arrive(&p_full);

@@ -310,6 +310,18 @@ def test_attend_many_rows_at_the_edges(D):
     check_attend(s, window=90)
 
 
+@pytest.mark.parametrize("ty,D", [("f16", 64), ("bf16", 128)])
+def test_attend_many_rows_scales_of_any_fraction(ty, D):
+    """Scales that are no powers of two, zeros and subnormals among V's: the same tolerance (an exponent off by
+    2^-16 at most is 1.1e-5 of a weight)."""
+    rng = np.random.default_rng(25)
+    s = attend_state(rng, [1000, 700], [200, 260], 8, 2, D, "e4m3", ty)
+    s["scales"] *= rng.uniform(1, 2, s["scales"].shape).astype(np.float32)
+    check_attend(s)
+    s["scales"][s["table"][0, 3], 0, 1], s["scales"][s["table"][1, 5], 1, 1] = 0.0, 1e-42
+    check_attend(s, window=300)
+
+
 def test_attend_many_rows_not_finite_scales():
     rng = np.random.default_rng(15)
     for which in (0, 1):
