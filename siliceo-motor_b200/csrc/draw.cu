@@ -386,7 +386,9 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
       run += w[j];
     }
   };
-  auto fast_bin = [&](float x) { return (top - x) * bin_scale; };
+  // The bin of a value, in every pass alike: what overflows (or is 0 times infinity) lies in the last one. Masked
+  // values fall there too; who looks at the last bin leaves them out.
+  auto fast_bin = [&](float x) { return fminf((top - x) * bin_scale, (float)(BINS - 1)); };
   // Rank 0: of the `count` places in sh.cand the last, in order, before which less than `goal` lies (`run` in
   // the places before all of them): weights, or numbers of places. Bins over the candidates' own range leave
   // few of them; those are put in order.
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
   if (by_k && p.top_k <= (int32_t)CAP / 2) {
     // At least top_k of the row's values reach the top_k-th largest of the threads' maxima, and few others
     // do: a histogram of the maxima alone gives the bin down to which all values are gathered.
-    if (mine_x > -INFINITY) atomicAdd(&sh.count[(uint32_t)fminf(fast_bin(mine_x), (float)(BINS - 1))], 1u);
+    if (mine_x > -INFINITY) atomicAdd(&sh.count[(uint32_t)fast_bin(mine_x)], 1u);
     if (tid == 0) sh.found[0] = ~0u;
     cl.sync();
     uint32_t c[4] = {}, all;
@@ -492,13 +494,13 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
       int bits = 0;
       if (round) while (((hi - lo) >> bits) >= BINS) bits++;
       auto bin_of = [&](float x, uint64_t pl) -> uint32_t {
-        return round ? (uint32_t)((hi - pl) >> bits) : (uint32_t)fminf(fast_bin(x), (float)(BINS - 1));
+        return round ? (uint32_t)((hi - pl) >> bits) : (uint32_t)fast_bin(x);
       };
       const bool everything = round == 0 && lo == 0;  // every value is in [lo, hi]: only its bin matters
       __syncthreads();
       if (everything) {
         each([&](float x, uint32_t) {
-          if (x > -INFINITY) atomicAdd(&sh.count[(uint32_t)fminf(fast_bin(x), (float)(BINS - 1))], 1u);
+          if (x > -INFINITY) atomicAdd(&sh.count[(uint32_t)fast_bin(x)], 1u);
         });
       } else {
         each([&](float x, uint32_t i) {
@@ -601,7 +603,7 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
                   const float b = fast_bin(x[j]);
                   ml += w[j];
                   ma += b < fa ? w[j] : 0;
-                  if (b >= fa && b < fb) {
+                  if (b >= fa && b < fb && x[j] > -INFINITY) {
                     mi += w[j];
                     collect(x[j], i + j);
                   }
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
 #pragma unroll 4
               for (uint32_t i = i0; i < i1; i++) {
                 const float x = value(vals[i]), b = fast_bin(x);
-                if (!(b >= f0 && b < fb)) continue;
+                if (!(b >= f0 && b < fb && x > -INFINITY)) continue;
                 const uint64_t w = wt.of(x);
                 if (b < fa) {
                   ma += w;
@@ -700,12 +702,13 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
         cl.sync();
         if (small && rank != 0) return;
         if (rank == 0) {
+          const uint32_t held = min(sh.n_cand, CAP);  // n_in, as both went by the same bins
           if (small) {
-            order((uint32_t)n_in);
-            draw_sorted((uint32_t)p.top_k);
+            order(held);
+            draw_sorted(min(held, (uint32_t)p.top_k));
             return;
           }
-          const uint64_t border = border_among((uint32_t)n_in, mass, above + (mass ? mass_above : n_above), mass ? goal : (double)p.top_k);
+          const uint64_t border = border_among(held, mass, above + (mass ? mass_above : n_above), mass ? goal : (double)p.top_k);
           if (tid == 0) sh.cut = border, sh.n_cand = 0;
         }
         cl.sync();

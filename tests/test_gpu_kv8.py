@@ -656,6 +656,28 @@ def test_draw_edges():
     check_draw(np.zeros((4, V)), [(1.0, 0, 1.0, 0.0)] * 4, np.array([1.0, -3.0, np.inf, np.nan], np.float32))
 
 
+@pytest.mark.parametrize("V", [300, 1000, 50000])
+@pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
+def test_draw_values_whose_distance_overflows(V, ty):
+    """Ordinary logits among some so far below the maximum that the distance in units of the temperature is no
+    finite f32, below the 1024 values that are ordered at once; an earlier draw left larger values everywhere."""
+    rng = np.random.default_rng(V + len(ty))
+    check_draw(rng.normal(30, 3, (40, 60000)), [(1.0, 500, 0.9, 0.0)] * 40, rng.random(40).astype(np.float32), ty)
+    params = [(1.0, k, p, 0.0) for k in (0, 20, 110, 200, 290, 590, 999) for p in (1.0, 0.9, 0.9999, 1 - 2.0**-23) if k or p < 1]
+    params += [(1e-37, 0, 0.9, 0.0), (1e-37, 250, 0.9, 0.0), (1e-37, 0, 1 - 2.0**-23, 0.1), (1e38, 0, 0.6, 0.0),
+               (1e38, 250, 1.0, 0.0), (float("inf"), 0, 0.7, 0.0), (float("inf"), 200, 0.99, 0.0)]
+    n, info = len(params), torch.finfo(TYPES[ty][0])
+    x = rng.normal(0, 2, (n, V))
+    x[np.arange(n), rng.integers(0, V, n)] = 12.0  # peaked
+    x = np.where(rng.random((n, V)) < 0.6, rng.choice([info.min, info.min / 2, -1e37 if ty != "f16" else -6e4], (n, V)), x)
+    x[::3, 7] = np.inf
+    x[1::3, 9] = info.max / 8
+    mask = None
+    if V > 1000:
+        mask = (rng.random((n, V)) < 600 / V).astype(np.uint8)
+    check_draw(x.astype(np.float32), params, rng.random(n).astype(np.float32), ty, mask=mask)
+
+
 def test_draw_largest_vocabulary():
     rng = np.random.default_rng(4)
     check_draw(rng.normal(0, 1, (6, 524288)).astype(np.float32), PARAMS[:6], rng.random(6).astype(np.float32))
