@@ -153,7 +153,8 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
   __shared__ uint64_t full_k[2], full_v[2], empty_k[2], empty_v[2], full_sc[4], s_full, p_full, pv_done, q_full, all_done;
   __shared__ float4 scales[4][2];  // of a step's pages: of K, of V, 1 if the page is there
   __shared__ ChunkPiece open_piece[2];
-  __shared__ uint32_t open_flag[2], last_flag[2], s_tmem, s_abort_word, s_gone;
+  __shared__ uint32_t open_flag[2], last_flag[2], s_tmem, s_abort_word;
+  __shared__ uint32_t s_gone[3];  // what the softmax warps agree on: a step's (two in turn), a piece's end
   volatile uint32_t* abort = &s_abort_word;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
@@ -379,10 +380,11 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
           if (warp == 0) {
             ch_wait<true>(&full_sc[it & 3], it / 4 & 1, a.err, abort);
             ch_wait<true>(&s_full, it & 1, a.err, abort);
-            if (lane == 0) s_gone = *abort;
+            // Two words in turn: the other warps may still be reading the last step's, and all must see the same.
+            if (lane == 0) s_gone[it & 1] = *abort;
           }
           ch_bar(1, CH_SOFT * 32);
-          gone = s_gone;
+          gone = s_gone[it & 1];
           if (gone) break;
           tc_fence_after();
           const int32_t p0 = step * (int32_t)CH_STEP;
@@ -482,10 +484,10 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
         if (!gone) {
           if (warp == 0) {
             ch_wait<true>(&pv_done, (it + 1) & 1, a.err, abort);
-            if (lane == 0) s_gone = *abort;
+            if (lane == 0) s_gone[2] = *abort;
           }
           ch_bar(1, CH_SOFT * 32);
-          gone = s_gone;
+          gone = s_gone[2];
         }
         tc_fence_after();
       }
