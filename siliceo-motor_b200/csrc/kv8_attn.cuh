@@ -8,10 +8,15 @@
 // t_j = log2 p_j and e_j = exponent of s_v(j): the weights of the products,
 // w_j = 2^(t_j + e_j - m + 13), are then relative to the largest
 // *contribution* and fit f16 whatever the spread of the pages' scales, while
-// the denominator adds w_j 2^-e_j in f32. m is kept a whole number, so moving
-// it multiplies by a power of two and rounds nothing. e_j is held to -60 .. 126,
-// so that 2^-e_j and sums of it stay in f32's range: smaller scales' weights
-// come out smaller instead.
+// the denominator adds 2^(t_j - m + 38) in f32. m is kept a whole number, so
+// moving it multiplies by a power of two and rounds nothing. e_j is held to
+// -60 .. 127: smaller scales' weights come out smaller instead. m is then at
+// most 128 above the largest t_j and at most 60 below it: the denominator's
+// terms and sums stay in f32's range (2^28 positions above, 2^-25 of the largest
+// term below). Both come from one exponential, 2^(t_j + g_j - m) with
+// g_j = max(e_j, 27): it is at most 2^87, and nothing of weight in the
+// denominator underflows however large another page's e is. Factors between
+// two maxima may be below 2^-126 and still count there (scaled).
 //
 // Bound by the cache bytes (2 hd a position and head): a warp copies a page at
 // a time into shared memory of its own, the next page's K under this page's
@@ -124,6 +129,17 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// The exponent of a V scale as the weights take it.
+__device__ __forceinline__ int v_exponent(uint32_t bits) { return min(max((int)(bits >> 23 & 255) - 127, -60), 127); }
+
+constexpr int SUM_EXP = 38;   // the denominator's exponent beside m
+constexpr int LIFT_FROM = 27;  // g = max(e, this)
+
+// x 2^d for whole d <= 0, given f = ex2(d), which is 0 below 2^-126.
+__device__ __forceinline__ float scaled(float x, float d, float f) {
+  return f == 0.f && x != 0.f ? x * 1.17549435e-38f * ex2(d + 126.f) : x * f;
+}
+
 // Codes 0, 1 and 2, 3 of a word as two f16 pairs.
 template <uint32_t FMT>
 __device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -177,6 +193,7 @@ template <uint32_t FMT, typename T, uint32_t HDV, uint32_t NR, bool FULL>
 __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_kernel(const Kv8AttnArgs a) {
   using L = Shape<T, HDV, NR>;
   constexpr bool SPLIT = L::SPLIT;
+  constexpr float SUM_UNIT = (float)(1u << (SUM_EXP - 13));  // the denominator's factor over the weights'
   constexpr uint32_t WARPS = L::WARPS, THREADS = WARPS * 32;
   constexpr int MT = HDV / 16, SEG = HDV / 64, NB = NR / 8;  // M tiles of O^T, 64-dim segments, n tiles of rows
   extern __shared__ __align__(128) float4 attn_smem4[];
@@ -431,9 +448,11 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
         if (has) {
           // ---- weights: s[nb][half][2 i + r] is position 16 half + 8 i + g, row 2t + r ----
           const float sk = __uint_as_float(sc.x), sv = __uint_as_float(sc.y);
-          const int ev = min(max((int)(sc.y >> 23 & 255) - 127, -60), 126);
-          // the weights' factor 2^13 comes with the scale's fraction and goes into l as well
-          const float e = (float)ev, back = __uint_as_float((uint32_t)(127 + 13 - ev) << 23), frac = sv * back;
+          const int ev = v_exponent(sc.y);
+          // the weights' factor 2^13 comes with the scale's fraction
+          const int gv = max(ev, LIFT_FROM);
+          const float e = (float)ev, lift = (float)(gv - ev), frac = sv * __uint_as_float((uint32_t)(127 + 13 - gv) << 23);
+          const float back = __uint_as_float((uint32_t)(127 + SUM_EXP - gv) << 23);
           const int32_t p0 = tile * (int32_t)TILE;
           const bool masked = p0 < all_lo || p0 + (int32_t)TILE > all_hi;
           float f[NB][2];
@@ -472,8 +491,8 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
                 x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
                 // whole: every factor between two maxima is exact
                 const float mn = fmaxf(m[nb][r], ceilf(x)), alpha = ex2(m[nb][r] - mn);
+                l[nb][r] = scaled(l[nb][r], m[nb][r] - mn, alpha);
                 m[nb][r] = mn;
-                l[nb][r] *= alpha;
 #pragma unroll
                 for (int j = 0; j < MT; j++) o[nb][j][r] *= alpha, o[nb][j][2 + r] *= alpha;
               }
@@ -486,7 +505,7 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
               float w[4];
 #pragma unroll
               for (int i = 0; i < 4; i++) {
-                const float y = ex2(s[nb][half][i] - m[nb][i & 1]);
+                const float y = ex2((s[nb][half][i] - m[nb][i & 1]) + lift);
                 sum[i & 1] += y;
                 w[i] = y * frac;
                 if (masked && s[nb][half][i] == -INFINITY) w[i] = 0.f;  // frac may be NaN
@@ -573,7 +592,7 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
           for (int r = 0; r < 2; r++) {
             const uint32_t in_block = nb * 8 + 2 * t + r, row = row_base + in_block;
             if (in_block >= rows || d0 >= hd) continue;
-            const float inv = l[nb][r] == 0.f ? 0.f : 1.f / l[nb][r];
+            const float inv = l[nb][r] == 0.f ? 0.f : SUM_UNIT / l[nb][r];
             T* dst = (T*)a.out + (uint64_t)(sq.row0 + row / a.group) * a.ld_out + (uint64_t)(head * a.group + row % a.group) * hd + d0;
             constexpr uint32_t PER = 16 / sizeof(T);
 #pragma unroll
@@ -608,7 +627,7 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
   __syncthreads();
 
   auto store = [&](const Piece& pc, uint32_t row, uint32_t d, float4 o, float l) {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : SUM_UNIT / l;
     const uint32_t r = pc.row_base + row;
     T* dst = (T*)a.out + (uint64_t)(pc.row0 + r / a.group) * a.ld_out + (uint64_t)(pc.head * a.group + r % a.group) * hd + d;
     if (d < hd) from_f(o.x * inv, dst[0]), from_f(o.y * inv, dst[1]), from_f(o.z * inv, dst[2]), from_f(o.w * inv, dst[3]);
@@ -638,6 +657,7 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
     for (uint32_t at = first_item; at < items; at += THREADS) {
       const uint32_t row = at / (HDV / 4), d = at % (HDV / 4) * 4;
       float m = MINM, l = 0.f;
+      bool lost = false;  // a factor of l was too small for it
       float4 o = make_float4(0, 0, 0, 0);
       for (uint32_t p = ids; p; p &= p - 1) m = fmaxf(m, L::part(attn_smem4, (__ffs(p) - 1) >> 1, (__ffs(p) - 1) & 1)[NR * HDV + row * 2]);
       for (uint32_t p = ids; p; p &= p - 1) {
@@ -645,8 +665,15 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
         const float2 ml = *reinterpret_cast<const float2*>(po + NR * HDV + row * 2);
         const float f = ex2(ml.x - m);
         const float4 v = *reinterpret_cast<const float4*>(po + row * HDV + d);
-        l += f * ml.y;
+        l += f * ml.y, lost |= f == 0.f && ml.y != 0.f;
         o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+      }
+      if (lost) {
+        l = 0.f;
+        for (uint32_t p = ids; p; p &= p - 1) {
+          const float* ml = L::part(attn_smem4, (__ffs(p) - 1) >> 1, (__ffs(p) - 1) & 1) + NR * HDV + row * 2;
+          l += scaled(ml[1], ml[0] - m, ex2(ml[0] - m));
+        }
       }
       if (whole) {
         store(pc, row, d, o, l);
@@ -687,6 +714,7 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
         const uint32_t way = at / ITEMS, row = at % ITEMS / (HDV / 4), d = at % (HDV / 4) * 4;
         if (row >= pc.rows) continue;
         float m = MINM, l = 0.f;
+        bool lost = false;
         float4 o = make_float4(0, 0, 0, 0);
         for (uint32_t c = way; c <= others; c += WAYS * 8) {
           float2 ml[8];
@@ -704,13 +732,21 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
 #pragma unroll
           for (uint32_t k = 0; k < 8; k++) mn = fmaxf(mn, ml[k].x);
           const float f0 = ex2(m - mn);
+          lost |= f0 == 0.f && l != 0.f;
           l *= f0, o.x *= f0, o.y *= f0, o.z *= f0, o.w *= f0;
           m = mn;
 #pragma unroll
           for (uint32_t k = 0; k < 8; k++) {
             const float f = ex2(ml[k].x - m);
-            l += f * ml[k].y;
+            l += f * ml[k].y, lost |= f == 0.f && ml[k].y != 0.f;
             o.x += f * v[k].x, o.y += f * v[k].y, o.z += f * v[k].z, o.w += f * v[k].w;
+          }
+        }
+        if (lost) {
+          l = 0.f;
+          for (uint32_t c = way; c <= others; c += WAYS) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part(c) + 16 * KV8_MAX_HD + row * 2));
+            l += scaled(ml.y, ml.x - m, ex2(ml.x - m));
           }
         }
         if (WAYS == 1) {
@@ -730,7 +766,7 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
           for (uint32_t w = 0; w < WAYS; w++) {
             const float f = ex2(ml_of[w][row].x - m);
             const float4 v = *reinterpret_cast<const float4*>(joint + (w * NR + row) * HDV + d);
-            l += f * ml_of[w][row].y;
+            l += scaled(ml_of[w][row].y, ml_of[w][row].x - m, f);
             o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
           }
           store(pc, row, d, o, l);

@@ -142,6 +142,7 @@ struct ChunkWalk {
 
 template <uint32_t FMT, typename T, uint32_t HD>
 __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnArgs a) {
+  constexpr float SUM_UNIT = (float)(1u << (SUM_EXP - 12));  // the denominator's factor over the weights'
   constexpr uint32_t CORE = 128 + 16;          // 16-byte columns of 8 rows, and a gap: see the decode warps
   constexpr uint32_t GROUP8 = HD / 8 * CORE;   // bytes of 8 positions
   constexpr uint32_t OPERAND = CH_STEP / 8 * GROUP8;  // bytes of a step's K or V
@@ -265,14 +266,14 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
         *reinterpret_cast<uint4*>(at) = lo;
         *reinterpret_cast<uint4*>(at + CORE) = hi;
       }
+      fence_proxy_async();
+      ch_arrive(&full[st]);
       if (brings) {
         // The slot's last readers, the softmax of step it - 4, are done: K's buffer came free after the scores
         // of step it - 2, which follow the weights of step it - 3.
         scales[it & 3][tid] = make_float4(sc.x, sc.y, there ? 1.f : 0.f, 0.f);
         ch_arrive(&full_sc[it & 3]);
       }
-      fence_proxy_async();
-      ch_arrive(&full[st]);
       it++;
     };
     // No early way out here: the four warps meet at a barrier each step, and after a wait that gave up
@@ -375,18 +376,9 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
           tc_fence_before();
           ch_arrive(&q_full);
         }
+        bool steep = false;  // some page's e is above 52
         for (int32_t step = pc.step; step < pc.stop && !gone; step++, it++) {
-          // one warp waits, the others for it at a barrier
-          if (warp == 0) {
-            ch_wait<true>(&full_sc[it & 3], it / 4 & 1, a.err, abort);
-            ch_wait<true>(&s_full, it & 1, a.err, abort);
-            // Two words in turn: the other warps may still be reading the last step's, and all must see the same.
-            if (lane == 0) s_gone[it & 1] = *abort;
-          }
-          ch_bar(1, CH_SOFT * 32);
-          gone = s_gone[it & 1];
-          if (gone) break;
-          tc_fence_after();
+          ch_wait<true>(&full_sc[it & 3], it / 4 & 1, a.err, abort);  // the scales come before the scores
           const int32_t p0 = step * (int32_t)CH_STEP;
           float f[2], e[2], back[2], frac[2];
           bool masked = p0 < pc.all_lo || p0 + (int32_t)CH_STEP > pc.all_hi;
@@ -394,11 +386,12 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             const float4 sc = scales[it & 3][h];
-            const int ev = min(max((int)(__float_as_uint(sc.y) >> 23 & 255) - 127, -60), 126);
-            // the weights' factor 2^12 comes with the scale's fraction and goes into l as well
+            const int ev = v_exponent(__float_as_uint(sc.y));
+            // the weights' factor 2^12 comes with the scale's fraction
             e[h] = (float)ev, back[h] = __uint_as_float((uint32_t)(127 + 12 - ev) << 23), frac[h] = sc.y * back[h];
             f[h] = mult * sc.x;
             here[h] = sc.z != 0.f;
+            steep |= e[h] > 52.f;
             masked |= !here[h] || !(frac[h] >= 4096.f && frac[h] < 8192.f);
           }
           // columns of this row that it sees: [lo, hi) of each page's 32
@@ -411,6 +404,16 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
               hi[h] = here[h] ? min(max(last_pos + 1 - (p0 + 32 * h), 0), 32) : 0;
             }
           }
+          // one warp waits, the others for it at a barrier
+          if (warp == 0) {
+            ch_wait<true>(&s_full, it & 1, a.err, abort);
+            // Two words in turn: the other warps may still be reading the last step's, and all must see the same.
+            if (lane == 0) s_gone[it & 1] = *abort;
+          }
+          ch_bar(1, CH_SOFT * 32);
+          gone = s_gone[it & 1];
+          if (gone) break;
+          tc_fence_after();
           float top = MINM;
           auto largest = [&](auto with_mask) {
 #pragma unroll
@@ -429,8 +432,8 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
           // Weights up to 2^14 fit f16 (times a scale's fraction): the maximum may lag by a factor 4.
           if (__any_sync(~0u, top - m > 2.f)) {
             const float mn = top - m > 2.f ? ceilf(top) : m, alpha = ex2(m - mn);
+            l = scaled(l, m - mn, alpha);
             m = mn;
-            l *= alpha;
             if (step != pc.step) {
 #pragma unroll 1
               for (uint32_t c = 0; c < HD / 32; c++) {
@@ -447,8 +450,12 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
 #pragma unroll
             for (int h = 0; h < 2; h++) {
               // Unmasked: the factor goes into the exponent (exact for a power of two; else off by 2^-16 at most, as
-              // |m| is at most 256) and out of l again (336 us; multiplying each weight 340).
-              const float c = e[h] - m + __log2f(frac[h]), lb = with_mask.value ? back[h] : __fdividef(back[h], frac[h]);
+              // |m| is at most 256) and out of l again (336 us; multiplying each weight 340). What underflows is
+              // nothing to l while no e is above 52.
+              const float c = e[h] - m + __log2f(frac[h]);
+              // Masked: 2^(t + g - m), as in the streaming form.
+              const float lift = fmaxf((float)LIFT_FROM - e[h], 0.f), low = ex2(-lift), fr = frac[h] * low;
+              const float lb = with_mask.value ? back[h] * SUM_UNIT * low : __fdividef(back[h] * SUM_UNIT, frac[h]);
               float sum = 0.f;
 #pragma unroll
               for (int half = 0; half < 2; half++) {
@@ -463,11 +470,14 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
                     const int col = 16 * half + 2 * i + j;
                     const bool see = !with_mask.value || (col >= lo[h] && col < hi[h]);
                     // large scores: t + e rounded as for the maximum, so that no weight passes 2^14
-                    if (with_mask.value) y[j] = ex2(fmaf(__uint_as_float(s[2 * i + j]), f[h], e[h]) - m);
-                    else y[j] = ex2(fmaf(__uint_as_float(s[2 * i + j]), f[h], c));
-                    if (!see) y[j] = 0.f;
-                    sum += y[j];
-                    if (with_mask.value) y[j] = see ? y[j] * frac[h] : 0.f;  // frac may be NaN
+                    if (with_mask.value) {
+                      y[j] = see ? ex2(fmaf(__uint_as_float(s[2 * i + j]), f[h], e[h]) - m + lift) : 0.f;
+                      sum += y[j];
+                      y[j] = see ? y[j] * fr : 0.f;  // fr may be NaN
+                    } else {
+                      y[j] = ex2(fmaf(__uint_as_float(s[2 * i + j]), f[h], c));
+                      sum += y[j];
+                    }
                   }
                   p[i] = pack_half(y[0], y[1]);
                 }
@@ -476,7 +486,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
               l = fmaf(sum, lb, l);
             }
           };
-          if (__any_sync(~0u, masked || fabsf(m) > 256.f)) weigh(std::true_type{}); else weigh(std::false_type{});
+          if (__any_sync(~0u, masked || steep || fabsf(m) > 256.f)) weigh(std::true_type{}); else weigh(std::false_type{});
           tmem_wait_st();
           tc_fence_before();
           ch_arrive(&p_full);
@@ -495,7 +505,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
       const bool whole = !pc.cut_left && !pc.cut_right, some = pc.step < pc.stop;
       const uint32_t side = pc.cut_left ? 0 : 1;
       float* gpart = a.part + ((uint64_t)blockIdx.x * 2 + side) * KV8_CHUNK_PART_FLOATS;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = l == 0.f ? 0.f : SUM_UNIT / l;
       T* dst = (T*)a.out + (uint64_t)(pc.row0 + token) * a.ld_out + (uint64_t)hq * HD;
 #pragma unroll 1
       for (uint32_t c = 0; c < HD / 16; c++) {
@@ -565,46 +575,52 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
     const ChunkPiece& p = open_piece[side];
     const int64_t c0 = p.unit / share;
     const uint32_t others = (uint32_t)((p.end - 1) / share - c0);
-    // A thread sums 8 dims of a row: all pieces' loads of up to eight are in flight at once.
+    auto part = [&](uint32_t c) { return a.part + ((uint64_t)(c0 + c) * 2 + (c ? 0 : 1)) * KV8_CHUNK_PART_FLOATS; };
+    auto ml_of = [&](uint32_t c, uint32_t row) { return __ldcg(reinterpret_cast<const float2*>(part(c) + CH_ROWS * KV8_MAX_HD) + row); };
+    // A thread a row: its maximum and the factor of its sum; then a thread 8 dims of a row, four pieces' loads in flight.
+    float2* of_row = reinterpret_cast<float2*>(ops);
+    if (side) __syncthreads();  // the first side's are read
+    if (threadIdx.x < p.rows) {
+      float m = MINM, l = 0.f;
+#pragma unroll 4
+      for (uint32_t c = 0; c <= others; c++) m = fmaxf(m, ml_of(c, threadIdx.x).x);
+#pragma unroll 4
+      for (uint32_t c = 0; c <= others; c++) {
+        const float2 ml = ml_of(c, threadIdx.x);
+        l += scaled(ml.y, ml.x - m, ex2(ml.x - m));
+      }
+      of_row[threadIdx.x] = make_float2(m, l == 0.f ? 0.f : SUM_UNIT / l);
+    }
+    __syncthreads();
     for (uint32_t at = threadIdx.x; at < p.rows * (HD / 8); at += CH_THREADS) {
       const uint32_t row = at / (HD / 8), d = at % (HD / 8) * 8;
-      float m = MINM, l = 0.f, o[8] = {};
+      const float2 mi = of_row[row];
+      float o[8] = {};
       for (uint32_t c = 0; c <= others; c += 4) {
-        float2 ml[4];
+        float f[4];
         float4 v[4][2];
 #pragma unroll
         for (uint32_t k = 0; k < 4; k++) {
-          ml[k] = make_float2(MINM, 0.f);
+          f[k] = MINM;
           v[k][0] = v[k][1] = make_float4(0, 0, 0, 0);
           if (c + k <= others) {
-            const float* part = a.part + ((uint64_t)(c0 + c + k) * 2 + (c + k ? 0 : 1)) * KV8_CHUNK_PART_FLOATS;
-            ml[k] = __ldcg(reinterpret_cast<const float2*>(part + CH_ROWS * KV8_MAX_HD) + row);
-            v[k][0] = __ldcg(reinterpret_cast<const float4*>(part + row * HD + d));
-            v[k][1] = __ldcg(reinterpret_cast<const float4*>(part + row * HD + d + 4));
+            f[k] = ml_of(c + k, row).x;
+            v[k][0] = __ldcg(reinterpret_cast<const float4*>(part(c + k) + row * HD + d));
+            v[k][1] = __ldcg(reinterpret_cast<const float4*>(part(c + k) + row * HD + d + 4));
           }
         }
-        float mn = m;
-#pragma unroll
-        for (uint32_t k = 0; k < 4; k++) mn = fmaxf(mn, ml[k].x);
-        const float f0 = ex2(m - mn);
-        l *= f0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) o[i] *= f0;
-        m = mn;
 #pragma unroll
         for (uint32_t k = 0; k < 4; k++) {
-          const float f = ex2(ml[k].x - m);
-          l += f * ml[k].y;
+          f[k] = ex2(f[k] - mi.x);
           const float* x = reinterpret_cast<const float*>(v[k]);
 #pragma unroll
-          for (int i = 0; i < 8; i++) o[i] += f * x[i];
+          for (int i = 0; i < 8; i++) o[i] += f[k] * x[i];
         }
       }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
       const uint32_t r = p.row_base + row;
       T v[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) from_f(o[i] * inv, v[i]);
+      for (int i = 0; i < 8; i++) from_f(o[i] * mi.y, v[i]);
       *reinterpret_cast<uint4*>((T*)a.out + (uint64_t)(p.row0 + r / a.group) * a.ld_out + (uint64_t)(p.head * a.group + r % a.group) * HD + d) =
           *reinterpret_cast<uint4*>(v);
     }

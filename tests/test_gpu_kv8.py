@@ -384,6 +384,38 @@ def test_attend_strides_scale_and_spread():
     check_attend(s)
 
 
+@pytest.mark.parametrize("ty,D,rows,length", [("f32", 64, 1, 300), ("f32", 128, 3, 9000), ("bf16", 128, 1, 9000),
+                                              ("bf16", 64, 20, 300), ("bf16", 64, 300, 900), ("bf16", 128, 256, 2500)])
+@pytest.mark.parametrize("low,high", [(-100, 66), (-60, 70), (-30, 90), (0, 118), (-20, 127)])
+def test_attend_scales_of_v_of_any_spread(ty, D, rows, length, low, high):
+    """A page of large values takes no part of the sum of weights away from pages whose scale is far smaller, in
+    whatever order and in whatever parts they are met (zeros come with the smallest scale, 2^-100).
+    Beside the tolerances above, weights x scale are f16 with the largest at 2^11 or more: a position is off by half
+    a subnormal step, 2^-25, which is 2^-36 of the largest p s_v, times its code (at most 127). That is what an
+    element is off by to which the largest page adds nothing."""
+    rng = np.random.default_rng(length + high)
+    pages = -(-length // 32)
+    for at in ([0], [pages - 1], [pages // 2, 1]):
+        s = attend_state(rng, [length, 33 + rows], [rows, rows], 4, 2, D, "i8", ty)
+        s["q"] *= 0.25
+        s["scales"][:, :, 1] = 2.0**low
+        if low == -100:
+            s["codes"][:, :, 1] = 0
+            big = s["table"][0, at]
+            s["codes"][big, :, 1] = rng.integers(-90, 91, s["codes"][big, :, 1].shape).astype(np.int8).view(np.uint8)
+        if high == 127:  # the largest that f32 holds: 2^127 x 1
+            s["codes"][:, :, 1] = np.clip(s["codes"][:, :, 1].view(np.int8), -1, 1).view(np.uint8)
+        s["scales"][s["table"][0, at], :, 1] = 2.0**high
+        got, q = call_attend(s), s["q"].double().numpy()
+        want, mag = ref.attend(s["codes"], s["scales"], "i8", q, s["lens"], s["first"], s["table"], D**-0.5)
+        flat = s["codes"].copy()  # V = 1 in the large pages, 0 elsewhere: their share of the sum is above their p
+        flat[:, :, 1] = s["scales"][:, :, 1, None, None] == 2.0**high
+        most = ref.attend(flat, s["scales"], "i8", q, s["lens"], s["first"], s["table"], D**-0.5)[0]
+        half, eps = {"f32": (2.0**-24, 2e-5), "bf16": (2.0**-8, 2.0**-11 + 2e-5)}[ty]
+        err = np.abs(got - want) - half * np.abs(want) - eps * mag - 2.0**-36 * 127 * length * most
+        assert np.all(err <= 2.0**-126), (at, float(err.max()))
+
+
 def test_attend_not_finite_scales_reach_the_rows_that_see_them():
     rng = np.random.default_rng(13)
     for which in (0, 1):
