@@ -390,7 +390,7 @@ int sm_kv_plan(uint64_t n_seqs, const int32_t* lens_dev, const int32_t* add_dev,
  * scale unless they need a larger one; the codes already there are then
  * rounded again, to the larger scale. Codes are rounded to nearest even. A row
  * that is not finite makes the scale of its page and head NaN, hence all those
- * values. */
+ * values. Codes and scales may not share bytes with other arguments. */
 int sm_kv8_append(const sm_kv8* c, const void* k_dev, const void* v_dev, uint32_t type, uint64_t n_rows, uint64_t ld_k,
                   uint64_t ld_v, const int64_t* slots_dev, void* stream);
 
@@ -416,7 +416,8 @@ int sm_kv8_ws_status(const sm_kv8_ws* w, void* stream);
  * row that sees nothing (a length of 0 or -1 among them) gets zeros, and rows
  * behind first_dev[n_seqs] are left as they were. Positions whose page id is
  * not in the pool take no part. Scales may be any finite values >= 0.
- * out may be q itself (with q's stride), or other columns of one matrix.
+ * out may be q itself (with q's stride), or other columns of one matrix; no
+ * other argument may lie between out's first byte and its last.
  * Products and sums are f32; scores and weights enter the tensor cores with
  * 22 bits for F32 rows and as f16 for F16 and BF16 rows. V scales below 2^-60
  * lose bits of them. */

@@ -84,9 +84,10 @@ void check_cache(Check& ck, const sm_kv8* c) {
   ck.want(c->n_kv_heads >= 1 && c->n_kv_heads <= 1024, "n_kv_heads must be 1..1024");
   ck.want(c->n_pages >= 1 && c->n_pages <= 0x7FFFFFFF, "n_pages must be 1..2^31 - 1");
 }
-void check_cache_memory(Check& ck, const sm_kv8* c) {
-  ck.ptr("codes_dev", c->codes_dev, 16);
-  ck.ptr("scales_dev", c->scales_dev, 8);
+void check_cache_memory(Check& ck, const sm_kv8* c, bool out) {
+  const uint64_t parts = c->n_pages * c->n_kv_heads * 2;
+  ck.ptr("codes_dev", c->codes_dev, 16, false, parts * KV8_PAGE * c->head_dim, out);
+  ck.ptr("scales_dev", c->scales_dev, 8, false, parts * sizeof(float), out);
 }
 
 Kv8 cache_of(const sm_kv8* c) {
@@ -153,10 +154,10 @@ int sm_kv8_append(const sm_kv8* c, const void* k_dev, const void* v_dev, uint32_
     if (!ld_v) ld_v = width;
     ck.want(ld_k >= width && ld_v >= width && ld_k < (1ull << 32) && ld_v < (1ull << 32), "a row stride is below n_kv_heads x head_dim, or 2^32 and above");
     ck.want(ld_k * es % 16 == 0 && ld_v * es % 16 == 0, "row strides must be multiples of 16 bytes");
-    check_cache_memory(ck, c);
-    ck.ptr("k_dev", k_dev, 16);
-    ck.ptr("v_dev", v_dev, 16);
-    ck.ptr("slots_dev", slots_dev, 8);
+    check_cache_memory(ck, c, true);
+    ck.ptr("k_dev", k_dev, 16, false, ((n_rows - 1) * ld_k + width) * es);
+    ck.ptr("v_dev", v_dev, 16, false, ((n_rows - 1) * ld_v + width) * es);
+    ck.ptr("slots_dev", slots_dev, 8, false, n_rows * 8);
     if (ck.memory()) return ck.rc;
     const cudaError_t e = launch_kv8_append(cache_of(c), k_dev, v_dev, type, (uint32_t)n_rows, ld_k, ld_v, slots_dev, (cudaStream_t)stream);
     return e == cudaSuccess ? SM_OK : cuda_error("sm_kv8_append", e);
@@ -244,7 +245,7 @@ int sm_kv8_attend(const sm_kv8* c, sm_kv8_ws* ws, const void* q_dev, void* out_d
     if (!ld_out) ld_out = width;
     ck.want(ld_q >= width && ld_out >= width && ld_q < (1ull << 32) && ld_out < (1ull << 32), "a row stride is below n_heads x head_dim, or 2^32 and above");
     ck.want(ld_q * es % 16 == 0 && ld_out * es % 16 == 0, "row strides must be multiples of 16 bytes");
-    check_cache_memory(ck, c);
+    check_cache_memory(ck, c, false);
     // Every row of q is read before it is written in out: they may be the same rows, or other columns of a matrix
     // that holds both, but must not overlap in another way.
     const uint64_t q0 = (uint64_t)(uintptr_t)q_dev, o0 = (uint64_t)(uintptr_t)out_dev, row = width * es;
@@ -254,10 +255,10 @@ int sm_kv8_attend(const sm_kv8* c, sm_kv8_ws* ws, const void* q_dev, void* out_d
       ck.want(ld_q == ld_out && (q0 == o0 || (apart >= row && apart <= pitch - row)), "out overlaps q other than row on row");
     }
     ck.ptr("q_dev", q_dev, 16);
-    ck.ptr("out_dev", out_dev, 16);
-    ck.ptr("lens_dev", lens_dev, 4);
-    ck.ptr("first_dev", first_dev, 4);
-    ck.ptr("table_dev", table_dev, 4, !table_ld);
+    ck.ptr("out_dev", out_dev, 16, false, o1 - o0, true);
+    ck.ptr("lens_dev", lens_dev, 4, false, n_seqs * 4);
+    ck.ptr("first_dev", first_dev, 4, false, (n_seqs + 1) * 4);
+    ck.ptr("table_dev", table_dev, 4, !table_ld, n_seqs * table_ld * 4);
     if (ck.memory()) return ck.rc;
     if (ws->device != ck.dev) return arg_error("sm_kv8_attend", "the workspace belongs to another device");
     Kv8AttnArgs a{};

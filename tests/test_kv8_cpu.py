@@ -103,6 +103,34 @@ def test_attend_refuses_rows_that_overlap_otherwise(kw, ok):
     assert ("overlaps" in str(e.value)) == (not ok)
 
 
+# A cache of 4 pages of 2 heads of 64: 32768 bytes of codes, 64 of scales. 9 f32 rows of K and V: 512 bytes each, of
+# q and out (4 heads): 1024. CTAs read K, V, slots, lengths and tables after others have written.
+@pytest.mark.parametrize("kw,ok", [
+    (dict(), True), (dict(k=A + 32752), False), (dict(k=A + 32768), True), (dict(v=A - 16), False),
+    (dict(v=A - 9 * 512), True), (dict(slots=2 * A), False), (dict(slots=2 * A - 64), False), (dict(slots=2 * A - 72), True),
+    (dict(slots=A + 8), False), (dict(scales=A + 32760), False), (dict(k=A - 9 * 512, ld_k=1024), False), (dict(v=3 * A), True)])
+def test_append_refuses_a_cache_over_other_arguments(kw, ok):
+    a = dict(codes=A, scales=2 * A, k=3 * A, v=4 * A, slots=5 * A)
+    a.update(kw)
+    c = cache(codes=a.pop("codes"), scales=a.pop("scales"))
+    with pytest.raises(smotor.EngineError) as e:  # where it takes them: there is no such memory
+        c.append(dtype=smotor.F32, n_rows=9, **a)
+    assert ("overlaps" in str(e.value)) == (not ok)
+
+
+@pytest.mark.parametrize("kw,ok", [
+    (dict(), True), (dict(out=A), False), (dict(out=A + 32768 - 16), False), (dict(out=A + 32768), True),
+    (dict(out=2 * A + 48), False), (dict(lens=4 * A + 9 * 1024 - 4), False), (dict(lens=4 * A + 9 * 1024), True),
+    (dict(lens=4 * A - 8), True), (dict(first=4 * A - 8), False), (dict(first=4 * A - 12), True),
+    (dict(table=4 * A - 28), False), (dict(table=4 * A - 32), True), (dict(lens=6 * A, first=6 * A), True),
+    (dict(lens=3 * A + 512), True), (dict(out=4 * A, ld_out=2048, lens=4 * A + 8 * 8192), False)])
+def test_attend_refuses_out_over_other_arguments(kw, ok):
+    a = dict(q=3 * A, out=4 * A, lens=5 * A, first=6 * A, table=7 * A, table_ld=4)
+    with pytest.raises(smotor.EngineError) as e:
+        cache(codes=A, scales=2 * A).attend(OneWorkspace, dtype=smotor.F32, n_rows=9, n_heads=4, n_seqs=2, **{**a, **kw})
+    assert ("overlaps" in str(e.value)) == (not ok)
+
+
 @pytest.mark.parametrize("kw", [dict(tokens=3 * A), dict(tokens=2 * A + 32), dict(tokens=A + 396), dict(logprobs=5 * A + 4),
                                 dict(logprobs=4 * A - 4), dict(ld=1 << 32), dict(tokens=4 * A, ld=128, mask=4 * A - 1123)])
 def test_draw_refuses_outputs_over_other_arguments(kw):
