@@ -369,7 +369,8 @@ typedef struct {
  *   table row or n_rows, or it needs pages and the pages that it and the
  *   sequences before it need are more than the list has. A refused sequence
  *   keeps its place in first_dev (a negative add counts as 0), takes no page,
- *   and its lens_out of -1 makes its rows attend to nothing.
+ *   and its lens_out of -1 makes its rows attend to nothing. It still holds
+ *   lens_dev[i] positions: that, not -1, is its length in the next step.
  * - status_dev [2]: pages left in the free list, number of refused sequences.
  * No output may share bytes with another argument (n_free_dev included). */
 int sm_kv_plan(uint64_t n_seqs, const int32_t* lens_dev, const int32_t* add_dev, int32_t* table_dev, uint64_t table_ld,

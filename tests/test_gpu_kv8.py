@@ -803,3 +803,56 @@ def test_serving_steps(fmt, ty, graph):
             assert int(tok[i]) == ref.draw(lg[i], 1.0, 40, float(np.float32(0.9)), float(np.float32(0.01)), float(u[i]))[0]
         lens.copy_(lens_out)
         n_free.copy_(status[:1])
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_serving_when_the_pool_runs_short(graph):
+    """A sequence that gets no pages keeps its length and its pages, and goes on when another one's are free."""
+    rng = np.random.default_rng(26)
+    n, H, Hq, D, P, ld, T = 3, 1, 2, 64, 6, 4, 120
+    i32 = dict(dtype=torch.int32, device="cuda")
+    codes, scales = torch.full((P, H, 2, 32, D), 0x7F, dtype=torch.uint8, device="cuda"), torch.zeros((P, H, 2), device="cuda")
+    table, free, n_free = torch.full((n, ld), -1, **i32), torch.arange(P, **i32), torch.tensor([P], **i32)
+    lens, lens_out, add, first = (torch.zeros(m, **i32) for m in (n, n, n, n + 1))
+    slots, status = torch.zeros(T, dtype=torch.int64, device="cuda"), torch.zeros(2, **i32)
+    k, v, q = (torch.zeros((T, h, D), device="cuda") for h in (H, H, Hq))
+    out = torch.zeros((T, Hq, D), device="cuda")
+    cache, ws = smotor.Kv8Cache(codes.data_ptr(), scales.data_ptr(), P, H, D), smotor.Kv8Workspace()
+
+    def step():
+        smotor.kv_plan(n, lens.data_ptr(), add.data_ptr(), table.data_ptr(), ld, free.data_ptr(), n_free.data_ptr(), T,
+                       lens_out.data_ptr(), first.data_ptr(), slots.data_ptr(), status.data_ptr(), stream=stream())
+        cache.append(k.data_ptr(), v.data_ptr(), smotor.F32, T, slots.data_ptr(), stream=stream())
+        cache.attend(ws, q.data_ptr(), out.data_ptr(), smotor.F32, T, Hq, n, lens_out.data_ptr(), first.data_ptr(),
+                     table.data_ptr(), ld, stream=stream())
+        lens.copy_(torch.where(lens_out >= 0, lens_out, lens))
+        n_free.copy_(status[:1])
+
+    g = None
+    if graph:
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            step()
+    held = []
+    for a in ([40, 33, 20], [30, 40, 1], [0, 40, 1], [0, 40, 1], [33, 1, 1]):
+        if len(held) == 3:  # the first sequence has ended
+            f, at = free.cpu().numpy(), int(n_free[0])
+            f[at:at + 3] = table[0, :3].cpu().numpy()
+            free.copy_(dev(f))
+            n_free += 3
+            lens[0] = 0
+        add.copy_(dev(np.array(a, np.int32)))
+        for x in (k, v, q):
+            x.copy_(dev(rng.normal(0, 1, x.shape).astype(np.float32)))
+        h = {m: x.cpu().numpy() for m, x in dict(lens=lens, table=table, free=free, codes=codes, scales=scales).items()}
+        want = ref.plan(h["lens"], a, h["table"], h["free"], int(n_free[0]), T)
+        (g.replay if g else step)()
+        torch.cuda.synchronize()
+        cw, sw = ref.append(h["codes"], h["scales"], k.double().cpu().numpy(), v.double().cpu().numpy(), want[3], "e4m3")
+        assert np.array_equal(codes.cpu().numpy(), cw) and np.array_equal(table.cpu().numpy(), want[0])
+        ow, mag = ref.attend(cw, sw, "e4m3", q.double().cpu().numpy(), want[1], want[2], want[0], D**-0.5)
+        R = int(want[2][-1])
+        assert np.all(np.abs(out.double().cpu().numpy()[:R] - ow[:R]) <= 2.0**-24 * np.abs(ow[:R]) + 2e-5 * mag[:R])
+        held.append(lens.tolist())
+    assert held == [[40, 33, 20], [70, 33, 21], [70, 33, 22], [0, 73, 23], [33, 74, 24]]
