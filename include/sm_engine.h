@@ -372,7 +372,8 @@ typedef struct {
  *   and its lens_out of -1 makes its rows attend to nothing. It still holds
  *   lens_dev[i] positions: that, not -1, is its length in the next step.
  * - status_dev [2]: pages left in the free list, number of refused sequences.
- * No output may share bytes with another argument (n_free_dev included). */
+ * No output may share bytes with another argument (n_free_dev included; of
+ * free_dev, whose length only the device knows, the first entry is checked). */
 int sm_kv_plan(uint64_t n_seqs, const int32_t* lens_dev, const int32_t* add_dev, int32_t* table_dev, uint64_t table_ld,
                const int32_t* free_dev, const int32_t* n_free_dev, uint64_t n_rows, int32_t* lens_out_dev,
                int32_t* first_dev, int64_t* slots_dev, int32_t* pos_dev, int32_t* seq_dev, int32_t* status_dev,
