@@ -62,6 +62,7 @@ struct Kv8AttnArgs {
   uint32_t window;                          // 0: none
   float scale;
   float* part;    // partial results, kv8_attn_part_floats()
+  float* keep;    // a CTA's products so far, kv8_attn_keep_floats()
   uint32_t* cnt;  // arrival counters, zero between launches, kv8_attn_counters()
   uint32_t* err;  // set when a bounded wait gave up
 };
@@ -91,6 +92,8 @@ constexpr uint32_t KV8_MAX_HD = 128;
 constexpr uint32_t KV8_PART_FLOATS = 16 * (KV8_MAX_HD + 2);  // a partial result of up to 16 rows: o, then m and l
 constexpr uint32_t KV8_CHUNK_PART_FLOATS = 128 * (KV8_MAX_HD + 2);  // the tensor-core form's (kv8_chunk.cuh, two CTAs an SM)
 inline uint64_t kv8_attn_part_floats(uint32_t sms) { return (uint64_t)sms * 2 * 2 * KV8_CHUNK_PART_FLOATS; }
+constexpr uint32_t KV8_KEEP_FLOATS = 16 * 68 * 32;  // of an SM: O and m of 16 warps' lanes, or O of two CTAs' 128 rows
+inline uint64_t kv8_attn_keep_floats(uint32_t sms) { return (uint64_t)sms * KV8_KEEP_FLOATS; }
 inline uint32_t kv8_attn_counters(uint32_t sms) { return sms * 2; }
 cudaError_t launch_kv8_attn_f32(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st);
 cudaError_t launch_kv8_attn_f16(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st);

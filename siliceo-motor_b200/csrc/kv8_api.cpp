@@ -16,7 +16,8 @@ using namespace sm;
 struct sm_kv8_ws {
   int device = 0;
   uint32_t sms = 0;
-  float* part = nullptr;
+  float* part = nullptr;  // partial results, then kept products
+  float* keep() const { return part + kv8_attn_part_floats(sms); }
   uint32_t* cnt = nullptr;  // the counters, then the error word
   uint32_t* err() const { return cnt + kv8_attn_counters(sms); }
 };
@@ -172,9 +173,9 @@ int sm_kv8_ws_new(sm_kv8_ws** out) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return cuda_error("sm_kv8_ws_new", e);
-    // One allocation, the counters and the error word behind the partial results. They are zeroed on a stream of
+    // One allocation, the counters and the error word behind the partial results and kept products. They are zeroed on a stream of
     // the call's own, so that no other work is waited for.
-    const size_t part = kv8_attn_part_floats((uint32_t)sms) * sizeof(float);
+    const size_t part = (kv8_attn_part_floats((uint32_t)sms) + kv8_attn_keep_floats((uint32_t)sms)) * sizeof(float);
     const size_t cnt = (kv8_attn_counters((uint32_t)sms) + 1) * sizeof(uint32_t);
     auto* w = new sm_kv8_ws;
     w->device = dev;
@@ -268,7 +269,7 @@ int sm_kv8_attend(const sm_kv8* c, sm_kv8_ws* ws, const void* q_dev, void* out_d
     a.n_seqs = (uint32_t)n_seqs, a.n_rows = (uint32_t)n_rows, a.n_heads = n_heads, a.group = n_heads / c->n_kv_heads;
     a.window = window;
     a.scale = scale;
-    a.part = ws->part, a.cnt = ws->cnt, a.err = ws->err();
+    a.part = ws->part, a.keep = ws->keep(), a.cnt = ws->cnt, a.err = ws->err();
     const cudaError_t e = launch_kv8_attn(a, type, ws->sms, (cudaStream_t)stream);
     return e == cudaSuccess ? SM_OK : cuda_error("sm_kv8_attend", e);
   });

@@ -60,6 +60,8 @@ namespace sm {
 namespace {
 
 constexpr uint32_t TILE = KV8_PAGE;  // positions of a step
+constexpr int32_t FOLD_FROM = 1024;  // pages of a unit that one warp adds up
+constexpr int32_t FOLD = 64;         // pages whose products the tensor core adds up before they are added in f32
 constexpr int32_t SHORT = 4;         // pages of a unit that is never cut: a merge would cost more
 constexpr float MINM = -3e38f;       // running maximum of a row that has seen nothing
 
@@ -189,7 +191,7 @@ __device__ __forceinline__ Seq seq_of(const Kv8AttnArgs& a, uint32_t s) {
   return q;
 }
 
-template <uint32_t FMT, typename T, uint32_t HDV, uint32_t NR, bool FULL>
+template <uint32_t FMT, typename T, uint32_t HDV, uint32_t NR, bool FULL, bool LONG>
 __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_kernel(const Kv8AttnArgs a) {
   using L = Shape<T, HDV, NR>;
   constexpr bool SPLIT = L::SPLIT;
@@ -412,6 +414,38 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
           for (int i = 0; i < 4; i++) o[nb][j][i] = 0.f;
         m[nb][0] = m[nb][1] = MINM, l[nb][0] = l[nb][1] = 0.f;
       }
+      // The tensor core cuts its sums off, all to one side: 1.3e-4 of O over 32768 positions of one sign, 5.5e-4
+      // over 131072. Where a warp may have more than FOLD_FROM pages of a unit (LONG), 16-bit rows' O goes to a sum
+      // in memory every FOLD pages, which is rounded: 1e-5 is left. Code that is there costs 3% where it does not
+      // run (4 sequences of up to 131072 positions, 28 pages a warp: 83.5 against 80.6 us), so it is a variant.
+      bool has_kept = false;
+      auto fold = [&](bool last) {  // the last into o itself
+        static_assert(NB * (MT * 4 + 2) * 32 * WARPS <= KV8_KEEP_FLOATS, "O and m of every lane");
+        float* kept = a.keep + (uint64_t)blockIdx.x * KV8_KEEP_FLOATS + warp * (NB * (MT * 4 + 2) * 32) + lane;
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++, kept += (MT * 4 + 2) * 32) {
+          float f[2] = {0.f, 0.f};
+#pragma unroll
+          for (int r = 0; r < 2; r++) {
+            if (has_kept) f[r] = ex2(kept[(MT * 4 + r) * 32] - m[nb][r]);
+            if (!last) kept[(MT * 4 + r) * 32] = m[nb][r];
+          }
+#pragma unroll
+          for (int j = 0; j < MT; j++) {
+            float was[4] = {0.f, 0.f, 0.f, 0.f};
+            if (has_kept) {
+#pragma unroll
+              for (int i = 0; i < 4; i++) was[i] = kept[(j * 4 + i) * 32];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              o[nb][j][i] = fmaf(was[i], f[i & 1], o[nb][j][i]);
+              if (!last) kept[(j * 4 + i) * 32] = o[nb][j][i], o[nb][j][i] = 0.f;
+            }
+          }
+        }
+        has_kept = true;
+      };
 
       for (; tile < tile_stop; tile++) {
         const uint32_t next = find(tile + 1);
@@ -572,7 +606,11 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
         __syncwarp();
         fetch_v(tile + 1, next);
         id = next;
+        if constexpr (LONG)
+          if (tile % FOLD == FOLD - 1 && tile + 1 < tile_stop) fold(false);
       }
+      if constexpr (LONG)
+        if (has_kept) fold(true);
       copy_wait<0>();
       // ---- this piece's result: lane (g, t) holds dims [d0, d0 + HDV / 8) of rows 2t, 2t + 1 ----
       const uint32_t d0 = HDV / 8 * g;
@@ -777,11 +815,18 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
   }
 }
 
-template <uint32_t FMT, typename T, uint32_t HDV, uint32_t NR, bool FULL>
+// Whether one of `shares` equal shares of the list, in units of `rows` rows, may hold more than FOLD_FROM pages of one.
+inline bool folds(const Kv8AttnArgs& a, uint32_t rows, uint32_t shares) {
+  const double units = ((double)a.n_rows * a.group / rows + a.n_seqs) * a.c.heads, pages = (double)a.table_ld;
+  return pages > FOLD_FROM && units * pages > (double)FOLD_FROM * shares;
+}
+template <uint32_t FMT, typename T, uint32_t HDV, uint32_t NR, bool FULL, bool LONG = false>
 cudaError_t attn_launch(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) {
   using L = Shape<T, HDV, NR>;
   static_assert(L::TOTAL <= 220 * 1024, "shared memory");
-  auto* kern = kv8_attn_kernel<FMT, T, HDV, NR, FULL>;
+  if constexpr (!L::SPLIT && !LONG)
+    if (folds(a, NR, sms * L::WARPS)) return attn_launch<FMT, T, HDV, NR, FULL, true>(a, sms, st);
+  auto* kern = kv8_attn_kernel<FMT, T, HDV, NR, FULL, LONG>;
   static SmemOnce once;
   const cudaError_t e = once.allow((const void*)kern, (int)L::TOTAL);
   if (e != cudaSuccess) return e;

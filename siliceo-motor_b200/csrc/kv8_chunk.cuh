@@ -48,6 +48,7 @@ namespace {
 constexpr uint32_t CH_ROWS = 128, CH_STEP = 64;
 constexpr uint32_t CH_SOFT = 4, CH_DEC = 8, CH_WARPS = CH_SOFT + CH_DEC + 1, CH_THREADS = CH_WARPS * 32;
 constexpr uint32_t CH_MIN_SHARE = 2;  // steps of a CTA
+constexpr int32_t CH_FOLD = FOLD;  // steps whose products the tensor core adds up before they are added in f32
 constexpr uint32_t CH_TCOLS = 256, CH_TS = 0, CH_TQ = 64, CH_TO = 128;  // tensor memory: S (and P over it), Q, O
 
 __device__ __forceinline__ void ch_arrive(uint64_t* b) {
@@ -140,7 +141,7 @@ struct ChunkWalk {
   }
 };
 
-template <uint32_t FMT, typename T, uint32_t HD>
+template <uint32_t FMT, typename T, uint32_t HD, bool LONG>
 __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnArgs a) {
   constexpr float SUM_UNIT = (float)(1u << (SUM_EXP - 12));  // the denominator's factor over the weights'
   constexpr uint32_t CORE = 128 + 16;          // 16-byte columns of 8 rows, and a gap: see the decode warps
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
         gone = __any_sync(~0u, !ok);
         if (gone) break;
         tc_fence_after();
-        const uint32_t more = step != pc.step;
+        const uint32_t more = step != pc.step && !(LONG && step % CH_FOLD == 0);
         if (ch_elect()) {
 #pragma unroll
           for (uint32_t k = 0; k < CH_STEP / 16; k++)
@@ -339,6 +340,10 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
     // ------------------------------------------------ softmax warps: a row a thread
     const uint32_t row = threadIdx.x, tl = tb + (warp * 32 << 16);
     const int64_t w64 = a.window ? (int64_t)a.window : (int64_t)1 << 40;
+    static_assert(2 * CH_ROWS * HD <= KV8_KEEP_FLOATS, "O of two CTAs");
+    float* kept = a.keep + (uint64_t)blockIdx.x * (CH_ROWS * HD) + row;  // of this row, dims CH_ROWS apart
+    float kept_m = MINM;
+    bool has_kept = false;
     bool gone = false;  // the CTA gave up: decided by the four warps as one, tensor-memory access is warp-wide
     while (walk.next(a, pc)) {
       float m = MINM, l = 0.f;
@@ -376,6 +381,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
           tc_fence_before();
           ch_arrive(&q_full);
         }
+        has_kept = false;
         bool steep = false;  // some page's e is above 52
         for (int32_t step = pc.step; step < pc.stop && !gone; step++, it++) {
           ch_wait<true>(&full_sc[it & 3], it / 4 & 1, a.err, abort);  // the scales come before the scores
@@ -429,12 +435,31 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
             }
           };
           if (masked) largest(std::true_type{}); else largest(std::false_type{});
+          // O so far to the kept sum; this step's product overwrites it.
+          const bool fold = LONG && step != pc.step && step % CH_FOLD == 0;
+          if (fold) {
+            const float fk = has_kept ? ex2(kept_m - m) : 0.f;
+#pragma unroll 1
+            for (uint32_t c = 0; c < HD / 16; c++) {
+              uint32_t o[16];
+              float was[16] = {}, *at = kept + 16 * c * CH_ROWS;
+              if (has_kept) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) was[i] = at[i * CH_ROWS];
+              }
+              tmem_ld16(tl + CH_TO + 16 * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; i++) at[i * CH_ROWS] = fmaf(was[i], fk, __uint_as_float(o[i]));
+            }
+            has_kept = true, kept_m = m;
+          }
           // Weights up to 2^14 fit f16 (times a scale's fraction): the maximum may lag by a factor 4.
           if (__any_sync(~0u, top - m > 2.f)) {
             const float mn = top - m > 2.f ? ceilf(top) : m, alpha = ex2(m - mn);
             l = scaled(l, m - mn, alpha);
             m = mn;
-            if (step != pc.step) {
+            if (step != pc.step && !fold) {
 #pragma unroll 1
               for (uint32_t c = 0; c < HD / 32; c++) {
                 uint32_t o[32];
@@ -513,6 +538,14 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
         if (some) {
           tmem_ld16(tl + CH_TO + 16 * c, o);
           tmem_wait_ld();
+          if (LONG && has_kept) {
+            const float fk = ex2(kept_m - m), *at = kept + 16 * c * CH_ROWS;
+            float was[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) was[i] = at[i * CH_ROWS];
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(fmaf(was[i], fk, __uint_as_float(o[i])));
+          }
         } else {
 #pragma unroll
           for (int i = 0; i < 16; i++) o[i] = 0;
@@ -627,10 +660,12 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
   }
 }
 
-template <uint32_t FMT, typename T, uint32_t HD>
+template <uint32_t FMT, typename T, uint32_t HD, bool LONG = false>
 cudaError_t chunk_launch(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) {
+  if constexpr (!LONG)
+    if (folds(a, CH_ROWS, 2 * sms)) return chunk_launch<FMT, T, HD, true>(a, sms, st);
   constexpr uint32_t smem = 4 * CH_STEP * HD * 2 / 128 * (128 + 16);  // four operands of columns CORE apart
-  auto* kern = kv8_chunk_kernel<FMT, T, HD>;
+  auto* kern = kv8_chunk_kernel<FMT, T, HD, LONG>;
   static SmemOnce once;
   const cudaError_t e = once.allow((const void*)kern, (int)smem);
   if (e != cudaSuccess) return e;

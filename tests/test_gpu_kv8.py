@@ -460,6 +460,47 @@ def test_attend_f32_keeps_its_bits_over_thousands_of_positions(fmt, D):
     assert np.linalg.norm(got - want) <= 4e-6 * np.linalg.norm(want)
 
 
+@pytest.mark.parametrize("rising", [False, True])
+@pytest.mark.parametrize("n,rows,D", [(300, 1, 128), (300, 1, 64), (150, 20, 128), (10, 400, 128), (10, 400, 64), (300, 1, 80)])
+def test_attend_16_bit_rows_over_long_caches(n, rows, D, rising):
+    """Sequences of 131072 positions, more than there are warps or CTAs to share one, over the same pages; V of one
+    sign. The mean of the signed errors: outputs are rounded to nearest, weights (f16) too, so what is left is the
+    tensor core's cut, 2^-23 of the sum a step of 16 positions, over the 128 steps (2048 positions) that it adds up by
+    itself: 1.5e-5, and as much again for a sum that has just passed a power of two. Over all 8192 steps it would be
+    up to 1e-3 (5.5e-4 was measured)."""
+    rng = torch.Generator(device="cuda").manual_seed(27)
+    H, L, dt = 8, 131072, torch.float16
+    P = L // 32
+    codes = torch.randint(0, 256, (P, H, 2, 32, D), generator=rng, dtype=torch.uint8, device="cuda")
+    codes[codes == 128] = 0
+    codes[:, :, 1] = torch.randint(64, 128, (P, H, 32, D), generator=rng, dtype=torch.uint8, device="cuda")
+    scales = torch.full((P, H, 2), 2.0**-7, device="cuda")
+    if rising:  # the largest contribution grows all the way
+        scales[:, :, 1] = 2.0 ** (-13 + torch.arange(P, device="cuda") * 12 // P)[:, None]
+    q = torch.randn((n * rows, H, D), generator=rng, device="cuda").to(dt)
+    out = torch.zeros_like(q)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    lens, first = torch.full((n,), L, **i32), torch.arange(n + 1, **i32) * rows
+    table = torch.arange(P, **i32).repeat(n, 1)
+    cache, ws = smotor.Kv8Cache(codes.data_ptr(), scales.data_ptr(), P, H, D, smotor.KV8_I8), smotor.Kv8Workspace()
+    cache.attend(ws, q.data_ptr(), out.data_ptr(), smotor.F16, n * rows, H, n, lens.data_ptr(), first.data_ptr(),
+                 table.data_ptr(), P, stream=stream())
+    ws.status(stream())
+    err = []
+    picks = torch.arange(0, n * rows, max(1, n * rows // 40), device="cuda")  # rows looked at
+    seen = L - rows + 1 + picks % rows
+    for h in range(H):
+        k = codes[:, h, 0].view(torch.int8).double().reshape(L, D) * 2.0**-7
+        v = (codes[:, h, 1].view(torch.int8).double() * scales[:, h, 1, None, None].double()).reshape(L, D)
+        t = q[picks, h].double() @ k.T * D**-0.5
+        t[torch.arange(L, device="cuda")[None] >= seen[:, None]] = -torch.inf
+        want = torch.softmax(t, 1) @ v
+        got = out[picks, h].double()
+        assert bool(((got - want).abs() <= (2.0**-11 + 2.0**-11 + 2e-5) * want).all())
+        err.append(((got - want) / want).mean())
+    assert abs(float(torch.stack(err).mean())) <= 3e-5
+
+
 @pytest.mark.parametrize("ty,rows", [("f32", 3), ("bf16", 1), ("f16", 20), ("bf16", 300)])
 @pytest.mark.parametrize("size", [1e9, 1e31])
 def test_attend_of_huge_scores(ty, rows, size):
