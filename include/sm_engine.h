@@ -426,7 +426,9 @@ int sm_kv8_ws_status(const sm_kv8_ws* w, void* stream);
  * steps are 2^-37 of it, so an element to which that page adds nothing keeps
  * less, and V scales below 2^-60 lose bits of their weights. Of F16 and BF16
  * rows up to 32768 positions are summed by the tensor core, which cuts sums off
- * (1.3e-4 where all V have one sign); longer ones are summed in parts. */
+ * (1.3e-4 where all V have one sign); longer ones are summed in parts. Scores
+ * must stay below f32's largest number. A row of q that is not finite gets NaN
+ * if it sees anything, and changes no other row. */
 int sm_kv8_attend(const sm_kv8* c, sm_kv8_ws* ws, const void* q_dev, void* out_dev, uint32_t type, uint64_t n_rows,
                   uint32_t n_heads, uint64_t ld_q, uint64_t ld_out, uint64_t n_seqs, const int32_t* lens_dev,
                   const int32_t* first_dev, const int32_t* table_dev, uint64_t table_ld, float scale, uint32_t window,

@@ -379,10 +379,11 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
         }
         top = max(top, __shfl_xor_sync(~0u, top, 1));
         top = max(top, __shfl_xor_sync(~0u, top, 2));
-        // The row times 2^k, its largest in [2^14, 2^15): f16 then holds what it can of every element.
+        // The row times 2^k, its largest in [2^14, 2^15): f16 then holds what it can of every element. A row that is
+        // not finite becomes NaN as a whole: scores of -inf would look like unseen ones.
         const int ex = (int)(top >> 23) - 127;
         const int k = top == 0 || ex == 128 ? 0 : min(14 - ex, 126);
-        const float up = __uint_as_float((uint32_t)(k + 127) << 23);
+        const float up = ex == 128 ? NAN : __uint_as_float((uint32_t)(k + 127) << 23);
         const float down = a.scale * 1.4426950408889634f / up;
 #pragma unroll
         for (int sg = 0; sg < SEG; sg++)

@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
       if (pc.step < pc.stop && !gone) {
         const int32_t last_pos = pc.pos0 + (int32_t)token;
         float mult;
-        {  // the row of Q, times a power of two that brings its largest to [2^14, 2^15), and the scale's sign
+        {  // the row of Q, times a power of two that brings its largest to [2^14, 2^15), and the scale's sign; or NaN
           const uint4* src = reinterpret_cast<const uint4*>((const T*)a.q + (uint64_t)(pc.row0 + token) * a.ld_q + (uint64_t)hq * HD);
           uint32_t top = 0;
 #pragma unroll 4
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
           }
           const int ex = (int)(top >> 23) - 127;
           const int k = top == 0 || ex == 128 ? 0 : min(14 - ex, 126);
-          const float up = __uint_as_float((uint32_t)(k + 127) << 23 | (__float_as_uint(a.scale) & 0x80000000u));
+          const float up = ex == 128 ? NAN : __uint_as_float((uint32_t)(k + 127) << 23 | (__float_as_uint(a.scale) & 0x80000000u));
           mult = a.scale * 1.4426950408889634f / up;
 #pragma unroll
           for (uint32_t c = 0; c < HD / 32; c++) {

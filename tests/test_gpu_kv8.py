@@ -425,6 +425,20 @@ def test_attend_not_finite_scales_reach_the_rows_that_see_them():
         assert np.isfinite(got[:2]).all() and np.isnan(got[2:40]).all() and np.isfinite(got[40]).all()
 
 
+@pytest.mark.parametrize("ty,D,rows", [("f32", 64, 3), ("f16", 64, 3), ("bf16", 80, 9), ("f16", 64, 300), ("bf16", 128, 260)])
+@pytest.mark.filterwarnings("ignore:invalid value")
+def test_attend_rows_that_are_not_finite(ty, D, rows):
+    """Of no use to others; NaN where they see something, however the signs fall, zeros where they do not."""
+    rng = np.random.default_rng(28)
+    s = attend_state(rng, [400, 2, 600], [rows, rows, 1], 4, 2, D, "i8", ty)
+    s["codes"][:, :, 0, :, 5] = 100  # K's dim 5: all scores of a row with an infinity there have one sign
+    for r, (h, d, x) in enumerate([(0, 5, np.inf), (1, 5, -np.inf), (2, 3, np.nan)]):
+        for base in (0, 2 * rows - 3, rows):  # the last rows of the second sequence see its two positions, its first none
+            s["q"][base + r, h, d] = float(x)
+    check_attend(s)
+    check_attend(s, window=1)
+
+
 def test_attend_repeats_bit_for_bit_and_on_another_stream():
     rng = np.random.default_rng(14)
     s = attend_state(rng, [3000, 10, 900], [1, 1, 2], 14, 2, 64, "e4m3", "f32")
