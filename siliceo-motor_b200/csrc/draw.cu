@@ -33,6 +33,7 @@
 #include <float.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8.cuh"
 
@@ -135,7 +136,8 @@ struct Weights {
   const double* table;  // 2^(43 + j / 16)
   double c, top;
   float floor;  // values below it weigh nothing
-  // A float in f64, by its bits (zero and subnormals come out as values below 2^-126: no weight changes by it).
+  // A float in f64, by its bits (zero and subnormals come out as values below 2^-126: no weight changes by it while
+  // c is below 2^81).
   static __device__ double wide(float x) {
     const uint32_t b = __float_as_uint(x);
     return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(b << 29));
@@ -217,8 +219,23 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const DrawArgs a, uint
     cl.sync();  // the others read post
     return;
   }
-  const float top = unordered((uint32_t)(best >> 32));
-  const double inv_t = 1.0 / (double)p.temperature;
+  float top = unordered((uint32_t)(best >> 32));
+  double inv_t = 1.0 / (double)p.temperature;
+  // At temperatures below 2^-80 zeros and subnormals differ from one another: row and temperature times 2^80, where
+  // the largest value is tiny itself. (Else only its equals weigh anything; and f16 holds nothing so small.)
+  if (sizeof(T) == 4 || std::is_same<T, __nv_bfloat16>::value) {
+    constexpr float up = 1.2089258e24f, far = -1.7014118e38f;  // 2^80, -2^127
+    if (p.temperature < 1.f / up && fabsf(top) < 9.0949470e-13f) {  // 2^-40
+      for (uint32_t i = tid; i < n; i += THREADS) {
+        const float x = load_logit(vals[i]);
+        if (x > -INFINITY) store_logit(fmaxf(x * up, far), vals[i]);
+      }
+      if (mine_x > -INFINITY) mine_x = fmaxf(mine_x * up, far);
+      top *= up, inv_t /= up;
+      best = (uint64_t)ordered(top) << 32 | (uint32_t)best;
+      __syncthreads();
+    }
+  }
   Weights wt;
   wt.table = sh.exp2_of;
   wt.c = inv_t * 1.4426950408889634074;

@@ -765,6 +765,19 @@ def test_draw_values_whose_distance_overflows(V, ty):
     check_draw(x.astype(np.float32), params, rng.random(n).astype(np.float32), ty, mask=mask)
 
 
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+def test_draw_tiny_temperatures(ty):
+    """Logits of the temperature's size down to the smallest floats, zeros and subnormal ones among them."""
+    rng = np.random.default_rng(29)
+    temps = [1e-20, 1e-26, 3e-30, 1e-36, 1e-37, 3e-38, 1e-38, 1e-39]
+    params = [(t, k, p, m) for t in temps for k, p, m in [(0, 1.0, 0.0), (40, 0.9, 0.0), (0, 0.7, 0.0), (0, 1.0, 0.2)]]
+    for shift in (0.0, -2.0, 3.0, 1e12):
+        t = np.array([q[0] for q in params])[:, None]
+        x = (rng.normal(0, 1.5, (len(params), 500)) + shift) * t
+        x[:, ::7] = 0.0 if shift < 1e12 else x[:, ::7]
+        check_draw(x.astype(np.float32), params, rng.random(len(params)).astype(np.float32), ty)
+
+
 def test_draw_largest_vocabulary():
     rng = np.random.default_rng(4)
     check_draw(rng.normal(0, 1, (6, 524288)).astype(np.float32), PARAMS[:6], rng.random(6).astype(np.float32))
