@@ -335,14 +335,14 @@ cudaError_t append_fmt(const Kv8& c, const void* k, const void* v, uint32_t type
 
 }  // namespace
 
-cudaError_t launch_kv8_plan(const Kv8PlanArgs& a, cudaStream_t st) {
+cudaError_t launch_kv8_plan(const Kv8PlanArgs& a, uint32_t sms, cudaStream_t st) {
   const size_t smem = (size_t)a.n_seqs * 8;
   if (smem > 40 * 1024) {
     static SmemOnce once;
     const cudaError_t e = once.allow((const void*)kv8_plan_kernel, KV8_PLAN_MAX_SEQS * 8);
     if (e != cudaSuccess) return e;
   }
-  const uint32_t grid = std::max(1u, std::min(148u, (uint32_t)(((uint64_t)a.n_rows + PLAN_ROWS - 1) / PLAN_ROWS)));
+  const uint32_t grid = std::max(1u, std::min(sms, (uint32_t)(((uint64_t)a.n_rows + PLAN_ROWS - 1) / PLAN_ROWS)));
   kv8_plan_kernel<<<grid, PLAN_THREADS, smem, st>>>(a);
   return cudaGetLastError();
 }

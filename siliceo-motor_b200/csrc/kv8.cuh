@@ -1,6 +1,6 @@
 // The 8-bit paged KV cache of hosts that batch their own requests: types and
-// launchers of its kernels (kv8.cu: page plan and append; kv8_attn.cu:
-// attention; draw.cu: the sampler that follows a step).
+// launchers of its kernels (kv8.cu: page plan and append; kv8_attn.cuh and
+// kv8_chunk.cuh: attention; draw.cu: the sampler that follows a step).
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -83,7 +83,7 @@ struct DrawArgs {
   uint32_t n_rows, vocab, type;
 };
 
-cudaError_t launch_kv8_plan(const Kv8PlanArgs& a, cudaStream_t st);
+cudaError_t launch_kv8_plan(const Kv8PlanArgs& a, uint32_t sms, cudaStream_t st);
 // ld_k, ld_v: elements between rows.
 cudaError_t launch_kv8_append(const Kv8& c, const void* k, const void* v, uint32_t type, uint32_t n_rows, uint64_t ld_k,
                               uint64_t ld_v, const int64_t* slots, cudaStream_t st);

@@ -136,7 +136,9 @@ int sm_kv_plan(uint64_t n_seqs, const int32_t* lens_dev, const int32_t* add_dev,
     if (ck.memory()) return ck.rc;
     Kv8PlanArgs a{lens_dev, add_dev, table_dev, table_ld, free_dev, n_free_dev, (uint32_t)n_seqs, (uint32_t)n_rows,
                   lens_out_dev, first_dev, slots_dev, pos_dev, seq_dev, status_dev};
-    const cudaError_t e = launch_kv8_plan(a, (cudaStream_t)stream);
+    int sms = 0;
+    cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, ck.dev);
+    if (e == cudaSuccess) e = launch_kv8_plan(a, (uint32_t)sms, (cudaStream_t)stream);
     return e == cudaSuccess ? SM_OK : cuda_error("sm_kv_plan", e);
   });
 }

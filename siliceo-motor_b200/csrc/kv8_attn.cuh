@@ -328,8 +328,8 @@ __global__ void __launch_bounds__(Shape<T, HDV, NR>::WARPS * 32, 1) kv8_attn_ker
         const uint32_t cpr = hd / 16, dst = ring + area;
 #pragma unroll
         for (uint32_t i = 0; i < HDV / 16; i++) {
-          if (!FULL && i >= cpr) break;
-          const uint32_t at = i * 32 + lane, row = FULL ? at / (HDV / 16) : at / cpr, col = at - row * (FULL ? HDV / 16 : cpr);
+          if (i >= cpr) break;
+          const uint32_t at = i * 32 + lane, row = at / cpr, col = at - row * cpr;
           copy16(dst + L::at(row, col), src + at * 16, (int32_t)row < n);
         }
       };

@@ -4,6 +4,6 @@
 
 namespace sm {
 cudaError_t launch_kv8_attn_f16(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) {
-  return chunk_takes<__half>(a) ? chunk_typed<__half>(a, sms, st) : attn_typed<__half>(a, sms, st);
+  return chunk_takes(a) ? chunk_typed<__half>(a, sms, st) : attn_typed<__half>(a, sms, st);
 }
 }  // namespace sm

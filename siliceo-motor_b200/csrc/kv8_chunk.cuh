@@ -676,8 +676,7 @@ cudaError_t chunk_launch(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) {
 // Rows of a sequence, on average, from which this form is taken: 4 sequences of 4096 positions, 8 KV heads, take
 // 54 us in the streaming form and 72 us in this one with 112 rows each, 108 us and 90 us with 300.
 constexpr uint32_t CHUNK_MIN_ROWS = 256;
-template <typename T>
-bool chunk_takes(const Kv8AttnArgs& a) {
+inline bool chunk_takes(const Kv8AttnArgs& a) {
   return (a.c.hd == 64 || a.c.hd == 128) && (uint64_t)a.n_rows * a.group >= (uint64_t)CHUNK_MIN_ROWS * a.n_seqs;
 }
 template <typename T>
