@@ -397,8 +397,10 @@ int sm_kv8_append(const sm_kv8* c, const void* k_dev, const void* v_dev, uint32_
                   uint64_t ld_v, const int64_t* slots_dev, void* stream);
 
 /* Scratch of sm_kv8_attend on the current device: partial results of
- * sequences that several CTAs share. One serves all calls that run one after
- * another; calls that may overlap (two streams, two graphs) need one each. */
+ * sequences that several CTAs share, and sums over long ones (60 MB on a B200).
+ * One serves all calls that run one after another; calls that may overlap (two
+ * streams, two graphs) need one each. Not to be made, freed or asked for its
+ * status while a stream is captured. */
 typedef struct sm_kv8_ws sm_kv8_ws;
 int sm_kv8_ws_new(sm_kv8_ws** out);
 int sm_kv8_ws_free(sm_kv8_ws* w);
@@ -434,7 +436,7 @@ int sm_kv8_attend(const sm_kv8* c, sm_kv8_ws* ws, const void* q_dev, void* out_d
                   const int32_t* first_dev, const int32_t* table_dev, uint64_t table_ld, float scale, uint32_t window,
                   void* stream);
 
-/* How sm_draw samples one row. */
+/* How sm_draw samples one row (the array of them is 16-byte aligned). */
 typedef struct {
   float temperature; /* > 0; else greedy: the largest logit, the lowest index among equals */
   int32_t top_k;     /* keep the k largest (equal ones: lowest indices first); <= 0: all */

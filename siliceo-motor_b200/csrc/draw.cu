@@ -24,9 +24,10 @@
 // barriers), by the f64 pipe where every weight is needed (top-p, min-p and
 // plain sampling: eleven operations a value). Measured on B200: one row of
 // 152064 f32 logits with top-k and top-p 14 us, with top-p alone 28 us, without
-// either 11 us; 64 rows of 128256 bf16 logits with settings of their own 58 us,
-// all with top-p 77 us: the rows run at once, two CTAs an SM, and the slowest
-// one's chain of passes and cluster barriers counts.
+// either 11 us; 64 rows of 128256 bf16 logits with settings of their own 57 us,
+// all with top-p 76 us: the rows run at once, two CTAs an SM (64 registers, 160
+// bytes of spill stores), and the slowest one's chain of passes and cluster
+// barriers counts.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

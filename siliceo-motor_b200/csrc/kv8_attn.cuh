@@ -40,12 +40,14 @@
 // shared memory, one cut between CTAs by the last of them to arrive.
 //
 // Measured on B200 (GPU time, launches back to back): 4 sequences of up to
-// 131072 positions, 28/4 heads of 128, bf16 rows, int8 codes: 81 us for 422 MB
-// (5.2 TB/s, 0.80 of the measured 6515 GB/s); 32 sequences of up to 4096, 32/8
+// 131072 positions, 28/4 heads of 128, bf16 rows, int8 codes: 80 us for 422 MB
+// (5.3 TB/s, 0.81 of the measured 6515 GB/s); 32 sequences of up to 4096, 32/8
 // heads: 47 us for 204 MB. The difference of the two is 6.4 TB/s, what is left
 // is about 15 us a launch: 3 us to the first copies, 2 to 5 to the first codes,
 // 5 to 9 of merging and of SMs that finish at different times. Row blocks of
-// up to 8 rows keep 16 warps an SM (128 registers); 16 rows 12 warps. Without
+// up to 8 rows keep 16 warps an SM (128 registers); 16 rows 12 warps. Some of
+// the state spills: 32 bytes a thread with 8 rows, 132 with 16, 92 for f32 rows
+// (head_dim 128; 39 and 262 local loads a scheduler in a launch). Without
 // the exchanged columns, copies by the lanes' own fragments took 12 shared
 // memory cycles more a page than the HBM time of the page.
 #pragma once
@@ -841,9 +843,12 @@ cudaError_t attn_hd(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) {
   return attn_launch<FMT, T, 128, NR, false>(a, sms, st);
 }
 // Units of 8 rows while that is what a sequence has on average (one token of a
-// group of up to 8 heads): half the registers, so more warps. Units of 16
-// read and decode the cache once for twice the rows. f32 rows: always 8, the
-// low halves take the registers.
+// group of up to 8 heads): half the registers, so more warps (32 sequences of
+// 3000, 8 KV heads of 128, 8 rows each: 47 against 55 us; of 64: 30 against 38).
+// Units of 16 read and decode the cache once for twice the rows (12 rows: 56.9
+// against 56.5 us, 24 rows 91 against 105; of 64: 39 and 40, 59 and 55). f32
+// rows: always 8, the low halves take the registers. The average is over what
+// the host knows: padding rows and idle sequences count.
 template <typename T>
 cudaError_t attn_typed(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {

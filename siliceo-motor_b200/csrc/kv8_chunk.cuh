@@ -28,13 +28,15 @@
 // leaves.
 //
 // Measured on B200: 2 sequences, chunks of up to 1024 rows over up to 8192
-// positions, 28/4 heads of 128, bf16 rows: 336 us, 480 TFLOP/s of what the rows
+// positions, 28/4 heads of 128, bf16 rows: 334 us, 482 TFLOP/s of what the rows
 // see (0.29 of the measured 1679); the streaming form takes 800. A step takes
-// an SM about 2200 cycles. The L1's data path is busy for 0.7 of them (scores
-// from tensor memory twice, weights back, operands written and read, codes),
-// the issue slots for 0.48, the tensor pipe for 0.2. A second S, its product
-// issued before the last step's weights are ready, with Q in shared memory,
-// hides the first product and still takes 364 us: the chain is not the bound.
+// an SM about 2200 cycles, and no unit is busy for all of them: the issue slots
+// 0.52, L1's data path 0.38, the tensor pipe 0.23. What counts is the softmax
+// warps' latency between a step's two products, which two CTAs an SM overlap
+// only in part. At 72 registers a thread they spill (196 bytes; 0.9 million
+// local loads a launch). A second S, its product issued before the last step's
+// weights are ready, with Q in shared memory, hides the first product and still
+// takes 364 us.
 #pragma once
 #include "kv8_attn.cuh"
 #include "tc_common.cuh"
@@ -475,7 +477,7 @@ __global__ void __launch_bounds__(CH_THREADS, 2) kv8_chunk_kernel(const Kv8AttnA
 #pragma unroll
             for (int h = 0; h < 2; h++) {
               // Unmasked: the factor goes into the exponent (exact for a power of two; else off by 2^-16 at most, as
-              // |m| is at most 256) and out of l again (336 us; multiplying each weight 340). What underflows is
+              // |m| is at most 256) and out of l again (4 us of 340 less than multiplying each weight). What underflows is
               // nothing to l while no e is above 52.
               const float c = e[h] - m + __log2f(frac[h]);
               // Masked: 2^(t + g - m), as in the streaming form.
@@ -673,8 +675,10 @@ cudaError_t chunk_launch(const Kv8AttnArgs& a, uint32_t sms, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// Rows of a sequence, on average, from which this form is taken: 4 sequences of 4096 positions, 8 KV heads, take
-// 54 us in the streaming form and 72 us in this one with 112 rows each, 108 us and 90 us with 300.
+// Rows of a sequence, on average, from which this form is taken. 4 sequences of 4096 positions in the streaming form
+// and in this one: 8 KV heads of 128, 62 and 78 us with 112 rows each, 76 and 73 with 160, 106 and 88 with 256, 185
+// and 108 with 512; 4 KV heads of 128, 40 and 53, 49 and 64, 65 and 82, 105 and 87; 8 of 64, 40 and 52, 50 and 54, 70
+// and 62, 122 and 81. The average is over what the host knows: padding rows and idle sequences count.
 constexpr uint32_t CHUNK_MIN_ROWS = 256;
 inline bool chunk_takes(const Kv8AttnArgs& a) {
   return (a.c.hd == 64 || a.c.hd == 128) && (uint64_t)a.n_rows * a.group >= (uint64_t)CHUNK_MIN_ROWS * a.n_seqs;
